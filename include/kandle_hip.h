@@ -500,6 +500,101 @@ int kh_gemv_fused(int prologue, const void* x, const void* x2, const void* norm_
 int kh_gemv_swiglu(int prologue, const void* x, const void* norm_w, float eps, const void* w_gu, int64_t ldw,
                    void* h, int64_t n_half, int64_t k, int x_dtype);
 
+/* ------------------------------------------------------------------ paged KV cache ----------- */
+
+/* A cache in pages: pools k_pages / v_pages [num_pages, hkv, page_size, d] (strides below, the d axis
+ * contiguous; page_size a power of two from 16 to 4096), a page table [batch, table_width] of device
+ * int32 page ids (row stride table_stride; an id outside [0, num_pages), by convention -1, is no page)
+ * and kv_lens [batch] (device int32): how many rows each sequence has cached, this call's new tokens
+ * among them.  Row p of sequence b lies in page page_table[b][p / page_size] at p % page_size.  The new
+ * tokens of all sequences are packed: sequence b's are rows query_starts[b] .. query_starts[b + 1] - 1
+ * (device int32 [batch + 1], nondecreasing) of the [tokens, heads, d] operands, and its last one is its
+ * last cached row; query_starts == NULL: one token per sequence (tokens == batch).  Nothing outside the
+ * operands is read or written whatever the device arrays hold.  The reference's cache is contiguous
+ * (packages/model-utils/src/kv-cache.ts:92-309); these entry points extend it to pages that sequences
+ * share and give back. */
+
+/* Attention of the new tokens over their sequences' cached rows: with n_b new tokens and L_b = kv_lens[b],
+ * token j of sequence b has position i = L_b - n_b + j and
+ *   o = sum_p softmax_p(scale q . k_p) v_p over the rows p <= i (causal) or p < L_b that lie below
+ *   max_kv_len and in a page;
+ * a token that sees no row is zero.  Query head h reads kv head h / (hq / hkv).  max_query_len: an upper
+ * bound of n_b (tokens j >= max_query_len are not computed); max_kv_len: an upper bound of L_b (rows at
+ * or behind it are not seen); both only size the launch, and INT64_MAX is always right.  Rows of o
+ * behind query_starts[batch] stay as they were.  `strides` (elements): q token, head; k page, head, row;
+ * v page, head, row; o token, head.  d 64 or 128, dtype KH_BF16 or KH_F32 (fp32 arithmetic throughout),
+ * q, pools and o 16-byte aligned with strides in 16-byte units.
+ * Extends flash_attention (reference: packages/types/src/backend/register.ts:102-109) to chunks behind a
+ * cached prefix and to ragged batches. */
+int kh_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
+                       const int32_t* kv_lens, const int32_t* query_starts, int64_t tokens, int64_t batch, int hq,
+                       int hkv, int d, int64_t num_pages, int64_t page_size, int64_t table_width,
+                       int64_t table_stride, const int64_t* strides, float scale, int causal, int64_t max_query_len,
+                       int64_t max_kv_len, int dtype);
+
+/* Writes the new tokens' k and v rows ([tokens, hkv, d], token and head strides) into their pages.  A token
+ * whose row lies outside the table or in no page is not written.  `strides` (elements): k token, head;
+ * v token, head; k_pages page, head, row; v_pages page, head, row.  Any d; rows on 16-byte boundaries
+ * are copied 16 bytes at a time.  Replaces kvCache.update's slice copies (reference:
+ * packages/model-utils/src/kv-cache.ts:164-212). */
+int kh_paged_kv_write(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
+                      const int32_t* kv_lens, const int32_t* query_starts, int64_t tokens, int64_t batch, int hkv, int d,
+                      int64_t num_pages, int64_t page_size, int64_t table_width, int64_t table_stride,
+                      const int64_t* strides, int dtype);
+
+/* Bookkeeping of the pages, on the device: page_refs [num_pages] (int32) counts the table entries that hold
+ * each page; a page is free while its count is 0.  Table entries behind a sequence's last row are -1.
+ * All four run under graph capture; every result is a function of the arguments alone. */
+
+/* Rows follow their parents: new_table[s] = page_table[parents[s]] and new_lens likewise (a parent outside
+ * [0, rows): an empty row, which frees it), and new_refs counts the new table's entries.  One call forks
+ * (a row with several children), reorders (beam search) and frees.  The results are contiguous and share
+ * no memory with the inputs.  No page is copied: kh_pages_reserve copies a shared tail when it grows. */
+int kh_pages_fork(const int32_t* page_table, int64_t table_stride, const int32_t* kv_lens, const int32_t* page_refs,
+                  const int32_t* parents, int64_t rows, int64_t table_width, int64_t num_pages, int32_t* new_table,
+                  int32_t* new_lens, int32_t* new_refs);
+
+/* Row s grows by counts[s] rows (<= 0: not at all), in place.  Its new pages are the lowest free ones, row
+ * after row.  A partly filled last page that other rows hold, too, is replaced by a new page, to which
+ * the caller copies it before it writes there: moves [rows, 2] receives these (from, to) pairs in row
+ * order and -1 behind them (kh_pages_copy takes them as they are); of several rows that grow on one page
+ * nobody else holds, the last keeps it.  info [3]: the number of moves; the pages that were missing; the
+ * rows that the table is too narrow for.  If either of the last two is not 0, nothing has changed.
+ * At most 2048 rows. */
+int kh_pages_reserve(int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int32_t* page_refs,
+                     const int32_t* counts, int64_t rows, int64_t table_width, int64_t num_pages, int64_t page_size,
+                     int32_t* moves, int32_t* info);
+
+/* Moves the live pages to the front of the pool: with n of them, the i-th live page at or behind n goes to
+ * the i-th free page before n.  new_table and new_refs (contiguous, no memory shared with the inputs)
+ * are the table and the counts afterwards; moves [max_moves, 2] (max_moves >= num_pages / 2) receives
+ * the (from, to) pairs for kh_pages_copy, and -1 behind them; info [2]: their number, and n. */
+int kh_pages_compact(const int32_t* page_table, int64_t table_stride, const int32_t* page_refs, int64_t rows,
+                     int64_t table_width, int64_t num_pages, int32_t* new_table, int32_t* new_refs, int32_t* moves,
+                     int64_t max_moves, int32_t* info);
+
+/* Copies whole pages: of each of `planes` contiguous pools [num_pages, page_bytes] (layers, keys and values),
+ * page moves[i][0] to page moves[i][1] for i < min(info[0], max_moves).  A pair with a page outside the
+ * pool is skipped; a destination must not be the source or destination of another pair.  page_bytes a
+ * multiple of 16, pages 16-byte aligned. */
+int kh_pages_copy(void* pages, int64_t planes, int64_t num_pages, int64_t page_bytes, const int32_t* moves,
+                  int64_t max_moves, const int32_t* info);
+
+/* The selection of a beam search step.  logits [groups, beams, vocab] (`strides`: group, beam, in elements;
+ * rows contiguous; KH_F32 or KH_BF16), scores [groups, beams] fp32:
+ *   score(g, b, t) = logits[g, b, t] - log(sum_t' exp logits[g, b, t']) + scores[g, b],
+ * a NaN logit or score counting as -inf, and all continuations of a beam whose score or sum is not finite
+ * being -inf.  With finished (int32 [groups, beams], may be NULL) a beam whose flag is not 0 has one
+ * continuation, the token eos at an unchanged score.  The k best of each group in order (the larger score,
+ * then the lower beam; inside a beam the larger logit, then the lower token): out_scores (fp32),
+ * out_tokens, out_parents (the beam, int32) and out_finished (given with finished: the parent's flag, or the
+ * token is eos), each [groups, k].  k <= 64, beams <= 64, k <= beams * vocab (with finished: k <= beams).
+ * Candidates are compared in float64.  Extends sample() (reference:
+ * packages/model-utils/src/sampling/index.ts:103-243) to several hypotheses. */
+int kh_beam_select(const void* logits, const int64_t* strides, const float* scores, const int32_t* finished, int64_t groups,
+                   int64_t beams, int64_t vocab, int k, int64_t eos, float* out_scores, int32_t* out_tokens,
+                   int32_t* out_parents, int32_t* out_finished, int dtype);
+
 #ifdef __cplusplus
 }
 #endif

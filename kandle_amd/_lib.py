@@ -90,6 +90,14 @@ SIGNATURES = {
     "kh_gemm_split_count": [_i64, _i64, _i64, C.POINTER(C.c_int)],
     "kh_gemm_split_count_for": [_i64, _i64, _i64, _i, C.POINTER(C.c_int)],
     "kh_gemm_splitk_partials": [_vp, _i64, _vp, _i64, _vp, _i64, _i64, _i64, _i, _i],
+    "kh_paged_attention": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _i, _i, _i64, _i64, _i64, _i64, _i64p, _f,
+                           _i, _i64, _i64, _i],
+    "kh_paged_kv_write": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _i, _i64, _i64, _i64, _i64, _i64p, _i],
+    "kh_pages_fork": [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp],
+    "kh_pages_reserve": [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp],
+    "kh_pages_compact": [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp],
+    "kh_pages_copy": [_vp, _i64, _i64, _i64, _vp, _i64, _vp],
+    "kh_beam_select": [_vp, _i64p, _vp, _vp, _i64, _i64, _i64, _i, _i64, _vp, _vp, _vp, _vp, _i],
     "kh_add_rms_norm": [_vp, _i, _i64, _vp, _vp, _vp, _i64, _i64, _f, _i],
 }
 

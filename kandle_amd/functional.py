@@ -84,6 +84,124 @@ def decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, seq_lens: Tens
 
 
 # ---------------------------------------------------------------------------------------------
+# paged KV cache and beam search
+# ---------------------------------------------------------------------------------------------
+def _limit(name: str, what: str, v) -> Optional[int]:
+    if v is None:
+        return None
+    if isinstance(v, bool) or int(v) != v or v < 0:
+        raise ValueError(f"{name}: {what} must be a non-negative integer, got {v!r}")
+    return int(v)
+
+
+def paged_attention(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_table: Tensor, kv_lens: Tensor,
+                    query_starts: Optional[Tensor] = None, scale: Optional[float] = None, is_causal: bool = True,
+                    max_query_len: Optional[int] = None, max_kv_len: Optional[int] = None,
+                    out: Optional[Tensor] = None) -> Tensor:
+    """Attention of new tokens over a paged KV cache: a chunk of a prompt, one token per sequence, or any
+    mixture of them.
+
+    query [T, Hq, D] packs the new tokens of B sequences, sequence b's being rows query_starts[b] ..
+    query_starts[b + 1] - 1 (int32 [B + 1]; None: one token each, T == B).  key_pages / value_pages
+    [pages, Hkv, page size, D] hold the cached rows, page_table (int32 [B, W]; -1: no page) says where,
+    kv_lens (int32 [B]) how many rows each sequence has, the new ones among them (write them first:
+    paged_kv_write).  Token j of n sits at position kv_lens[b] - n + j and sees the rows up to its own
+    (is_causal) or all kv_lens[b] of them, except those in no page; a token that sees none is zero.  GQA
+    as scaled_dot_product_attention, scale 1/sqrt(D) by default.  float32 or bfloat16, D 64 or 128, page size a
+    power of two from 16 to 4096.
+
+    max_query_len and max_kv_len, upper bounds of the new tokens and cached rows of a sequence, keep the launch
+    small; tokens and rows beyond them are left out.  Rows of `out` behind the last sequence stay as they
+    were (a new result's are undefined)."""
+    if scale is None:
+        scale = 1.0 / math.sqrt(query.shape[-1])
+    output = out.handle if out is not None else _new(query, query.shape)
+    _kernel(query, "paged_attention")(query.handle, key_pages.handle, value_pages.handle, page_table.handle, kv_lens.handle,
+                                      query_starts.handle if query_starts is not None else None, output, float(scale),
+                                      bool(is_causal), _limit("paged_attention", "max_query_len", max_query_len),
+                                      _limit("paged_attention", "max_kv_len", max_kv_len))
+    return out if out is not None else _wrap(output)
+
+
+def paged_kv_write(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Tensor, page_table: Tensor,
+                   kv_lens: Tensor, query_starts: Optional[Tensor] = None) -> None:
+    """Writes the new tokens' key and value rows [T, Hkv, D] into the pages that paged_attention will read
+    them from (same page_table, kv_lens and query_starts).  A row without a page is not written."""
+    _kernel(key, "paged_kv_write")(key.handle, value.handle, key_pages.handle, value_pages.handle, page_table.handle,
+                                   kv_lens.handle, query_starts.handle if query_starts is not None else None)
+
+
+def pages_fork(page_table: Tensor, kv_lens: Tensor, page_refs: Tensor, parents: Tensor, out=None):
+    """(page_table, kv_lens, page_refs) after every row has taken over its parent's pages: row s those of
+    parents[s] (int32 [rows]; -1: none, the row is freed).  Pages are shared, not copied; page_refs (int32
+    [pages]) counts their holders.  out: the three results, which share no memory with the inputs."""
+    if out is None:
+        out = (_wrap(_new(page_table, page_table.shape)), _wrap(_new(kv_lens, kv_lens.shape)),
+               _wrap(_new(page_refs, page_refs.shape)))
+    table, lens, refs = out
+    _kernel(page_table, "pages_fork")(page_table.handle, kv_lens.handle, page_refs.handle, parents.handle, table.handle,
+                                      lens.handle, refs.handle)
+    return table, lens, refs
+
+
+def pages_reserve(page_table: Tensor, kv_lens: Tensor, page_refs: Tensor, counts: Tensor, page_size: int, out=None):
+    """Grows row s of the page table by counts[s] rows (int32; <= 0: not at all) in place: kv_lens, the new
+    pages (the lowest free ones, row after row) and page_refs.  A partly filled last page that other rows hold,
+    too, is replaced; its contents have to follow: pages_copy(pages, moves, info).
+
+    Returns (moves int32 [rows, 2], info int32 [3]): pairs (from, to), and their number, the pages that were
+    missing and the rows that the table is too narrow for.  If any were, nothing has changed."""
+    if out is None:
+        rows = page_table.shape[0]
+        out = (_wrap(_new(page_table, (rows, 2))), _wrap(_new(page_table, (3,))))
+    moves, info = out
+    _kernel(page_table, "pages_reserve")(page_table.handle, kv_lens.handle, page_refs.handle, counts.handle, int(page_size),
+                                         moves.handle, info.handle)
+    return moves, info
+
+
+def pages_compact(page_table: Tensor, page_refs: Tensor, out=None):
+    """(page_table, page_refs, moves, info) for the live pages moved to the front of the pool; the pages follow with
+    pages_copy(pages, moves, info).  moves int32 [max(1, pages // 2), 2], info int32 [2]: the number of moves, and of
+    live pages.  out: the four results; the first two share no memory with the inputs."""
+    if out is None:
+        n = max(1, page_refs.shape[0] // 2)
+        out = (_wrap(_new(page_table, page_table.shape)), _wrap(_new(page_refs, page_refs.shape)),
+               _wrap(_new(page_table, (n, 2))), _wrap(_new(page_table, (2,))))
+    table, refs, moves, info = out
+    _kernel(page_table, "pages_compact")(page_table.handle, page_refs.handle, table.handle, refs.handle, moves.handle, info.handle)
+    return table, refs, moves, info
+
+
+def pages_copy(pages: Tensor, moves: Tensor, info: Tensor) -> Tensor:
+    """Copies page moves[i, 0] to page moves[i, 1] for i < info[0] in every pool of `pages` [..., num_pages, Hkv,
+    page size, D] (layers, keys and values at once).  No page may be written twice, or written and read."""
+    _kernel(pages, "pages_copy")(pages.handle, moves.handle, info.handle)
+    return pages
+
+
+def beam_select(logits: Tensor, scores: Tensor, k: Optional[int] = None, finished: Optional[Tensor] = None,
+                eos_token_id: Optional[int] = None, out=None):
+    """The k (default: as many as there are beams) best continuations of every group of beams: logits [groups,
+    beams, vocab] (float32 or bfloat16), scores [groups, beams] (float32: the beams' log-probabilities so
+    far), finished (int32 [groups, beams], optional): beams that have ended, which go on as themselves, with
+    eos_token_id, at their score.
+
+    Returns (scores, tokens, parents, finished), each [groups, k] and best first: log_softmax(logits)[token] +
+    scores[parent], ties to the lower beam and token; finished is None without flags given."""
+    groups, beams = logits.shape[0], logits.shape[1]
+    k = beams if k is None else int(k)
+    if out is None:
+        new = lambda dtype: _wrap(_new(scores, (groups, k), dtype))  # noqa: E731
+        out = (new("float32"), new("int32"), new("int32"), new("int32") if finished is not None else None)
+    o_scores, o_tokens, o_parents, o_finished = out
+    _kernel(logits, "beam_select")(logits.handle, scores.handle, finished.handle if finished is not None else None, k,
+                                   eos_token_id if finished is not None else None, o_scores.handle, o_tokens.handle,
+                                   o_parents.handle, o_finished.handle if o_finished is not None else None)
+    return o_scores, o_tokens, o_parents, o_finished
+
+
+# ---------------------------------------------------------------------------------------------
 # matmul / linear
 # ---------------------------------------------------------------------------------------------
 def dispatch_matmul(a: Tensor, b: Tensor, c: Optional[Tensor] = None, alpha: float = 1.0, beta: float = 0.0,

@@ -16,6 +16,9 @@ New fused names (no reference schema; the reference composes them from the ops a
   rms_norm_rope(q, k, params) -> (q_out, k_out)   qk-norm + RoPE (+ V cache write)
   silu_mul(gate, up, output) -> None              SwiGLU activation
   decode_attention(q, k_cache, v_cache, seq_lens, output, scale) -> None   varlen split-K decode
+  paged_attention / paged_kv_write      new tokens of a ragged batch over, and into, a paged KV cache
+  pages_fork / _reserve / _compact / _copy   the pages' bookkeeping, on the device
+  beam_select                           the best continuations of groups of beams
 """
 from __future__ import annotations
 
@@ -1105,7 +1108,204 @@ def philox4x32_10(seed: int, counters, out) -> None:
               _vp(out.data_ptr()))
 
 
+# ---------------------------------------------------------------------------------------------
+# paged KV cache
+# ---------------------------------------------------------------------------------------------
+_NO_LIMIT = (1 << 63) - 1
+
+
+def _int32(name: str, what: str, h, shape) -> None:
+    """An int32 tensor of `shape` with contiguous data."""
+    if h.dtype != INT32 or h.shape != shape or not h.is_contiguous():
+        raise ValueError(f"{name}: {what} must be a contiguous int32 tensor of shape {list(shape)}, got "
+                         f"{h.dtype} {list(h.shape)}")
+
+
+def _page_table(name: str, table) -> None:
+    if table.dtype != INT32 or len(table.shape) != 2 or (table.shape[1] > 1 and table.strides[1] != 1):
+        raise ValueError(f"{name}: page_table must be an int32 tensor [sequences, pages] with contiguous rows, got "
+                         f"{table.dtype} {list(table.shape)}")
+    if table.shape[0] > 1 and table.strides[0] < table.shape[1]:
+        raise ValueError(f"{name}: page_table's rows must not overlap")
+
+
+def _row_stride(table) -> int:
+    return table.strides[0] if table.shape[0] > 1 else table.shape[1]
+
+
+def _token_rows(name: str, what: str, h, heads: int, d: int) -> list:
+    """(token, head) strides of a [tokens, heads, d] tensor with contiguous rows."""
+    if len(h.shape) != 3 or h.shape[1] != heads or h.shape[2] != d or not (_last_dim_contiguous(h)):
+        raise ValueError(f"{name}: {what} must be [tokens, {heads}, {d}] with a contiguous last dim, got {list(h.shape)}")
+    return [h.strides[0], h.strides[1]]
+
+
+def _pools(name: str, k_pages, v_pages) -> list:
+    ks = k_pages.shape
+    if len(ks) != 4 or v_pages.shape != ks or not _last_dim_contiguous(k_pages) or not _last_dim_contiguous(v_pages):
+        raise ValueError(f"{name}: key and value pages must be [pages, kv heads, page size, head dim] alike with a contiguous "
+                         f"last dim, got {list(ks)} and {list(v_pages.shape)}")
+    return list(k_pages.strides[:3]) + list(v_pages.strides[:3])
+
+
+def _sequences(name: str, table, kv_lens, query_starts, tokens: int) -> int:
+    """The batch size; the arrays' shapes checked."""
+    _page_table(name, table)
+    B = table.shape[0]
+    _int32(name, "kv_lens", kv_lens, (B,))
+    if query_starts is not None:
+        _int32(name, "query_starts", query_starts, (B + 1,))
+    elif tokens != B:
+        raise ValueError(f"{name}: without query_starts every sequence has one new token ({tokens} tokens, {B} sequences)")
+    return B
+
+
+def paged_attention(query, key_pages, value_pages, page_table, kv_lens, query_starts, output, scale: float,
+                    is_causal: bool, max_query_len=None, max_kv_len=None) -> None:
+    """Attention of a ragged batch's new tokens over a paged cache (kh_paged_attention): query / output
+    [tokens, Hq, D], pools [pages, Hkv, page size, D], page_table int32 [B, W], kv_lens int32 [B],
+    query_starts int32 [B + 1] or None (one token each).  Rows behind the last sequence stay as they were."""
+    dt = query.dtype
+    if dt not in (FLOAT32, BFLOAT16) or key_pages.dtype != dt or value_pages.dtype != dt or output.dtype != dt:
+        raise TypeError(f"paged_attention: query, pages and output must share float32 or bfloat16, got {dt}, "
+                        f"{key_pages.dtype}, {value_pages.dtype}, {output.dtype}")
+    pools = _pools("paged_attention", key_pages, value_pages)
+    n_pages, hkv, page, d = key_pages.shape
+    if len(query.shape) != 3:
+        raise ValueError(f"paged_attention: query must be [tokens, heads, head dim], got {list(query.shape)}")
+    tokens, hq, _ = query.shape
+    qs = _token_rows("paged_attention", "query", query, hq, d)
+    os_ = _token_rows("paged_attention", "output", output, hq, d)
+    if output.shape[0] != tokens:
+        raise ValueError(f"paged_attention: output has {output.shape[0]} tokens, query {tokens}")
+    if hkv == 0 or hq % hkv != 0:
+        raise ValueError(f"paged_attention: numHeadsQ ({hq}) must be divisible by numHeadsKV ({hkv})")
+    if not math.isfinite(scale):
+        raise ValueError(f"paged_attention: scale {scale} is not finite")
+    B = _sequences("paged_attention", page_table, kv_lens, query_starts, tokens)
+    _lib.call("kh_paged_attention", query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), output.data_ptr(),
+              page_table.data_ptr(), kv_lens.data_ptr(), None if query_starts is None else query_starts.data_ptr(), tokens, B,
+              hq, hkv, d, n_pages, page, page_table.shape[1], _row_stride(page_table),
+              _lib.i64_array(qs + pools + os_), scale, 1 if is_causal else 0,
+              _NO_LIMIT if max_query_len is None else max_query_len, _NO_LIMIT if max_kv_len is None else max_kv_len,
+              query.kh_dtype)
+
+
+def paged_kv_write(key, value, key_pages, value_pages, page_table, kv_lens, query_starts) -> None:
+    """The new tokens' rows key / value [tokens, Hkv, D] into their pages (kh_paged_kv_write)."""
+    dt = key.dtype
+    if dt not in (FLOAT32, BFLOAT16) or value.dtype != dt or key_pages.dtype != dt or value_pages.dtype != dt:
+        raise TypeError(f"paged_kv_write: rows and pages must share float32 or bfloat16, got {dt}, {value.dtype}, "
+                        f"{key_pages.dtype}, {value_pages.dtype}")
+    pools = _pools("paged_kv_write", key_pages, value_pages)
+    n_pages, hkv, page, d = key_pages.shape
+    st = _token_rows("paged_kv_write", "key", key, hkv, d) + _token_rows("paged_kv_write", "value", value, hkv, d)
+    tokens = key.shape[0]
+    if value.shape[0] != tokens:
+        raise ValueError(f"paged_kv_write: key has {tokens} tokens, value {value.shape[0]}")
+    B = _sequences("paged_kv_write", page_table, kv_lens, query_starts, tokens)
+    _lib.call("kh_paged_kv_write", key.data_ptr(), value.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
+              page_table.data_ptr(), kv_lens.data_ptr(), None if query_starts is None else query_starts.data_ptr(), tokens, B,
+              hkv, d, n_pages, page, page_table.shape[1], _row_stride(page_table), _lib.i64_array(st + pools), key.kh_dtype)
+
+
+def _page_refs(name: str, page_refs) -> int:
+    if page_refs.dtype != INT32 or len(page_refs.shape) != 1 or not page_refs.is_contiguous():
+        raise ValueError(f"{name}: page_refs must be a contiguous int32 tensor [pages], got {page_refs.dtype} {list(page_refs.shape)}")
+    return page_refs.shape[0]
+
+
+def pages_fork(page_table, kv_lens, page_refs, parents, new_table, new_lens, new_refs) -> None:
+    """Rows of a page table follow their parents (kh_pages_fork)."""
+    _page_table("pages_fork", page_table)
+    rows, width = page_table.shape
+    n = _page_refs("pages_fork", page_refs)
+    for what, h in (("kv_lens", kv_lens), ("parents", parents), ("the new kv_lens", new_lens)):
+        _int32("pages_fork", what, h, (rows,))
+    _int32("pages_fork", "the new page_table", new_table, (rows, width))
+    _int32("pages_fork", "the new page_refs", new_refs, (n,))
+    _lib.call("kh_pages_fork", page_table.data_ptr(), _row_stride(page_table), kv_lens.data_ptr(), page_refs.data_ptr(),
+              parents.data_ptr(), rows, width, n, new_table.data_ptr(), new_lens.data_ptr(), new_refs.data_ptr())
+
+
+def pages_reserve(page_table, kv_lens, page_refs, counts, page_size: int, moves, info) -> None:
+    """Rows of a page table grow, in place (kh_pages_reserve)."""
+    _page_table("pages_reserve", page_table)
+    rows, width = page_table.shape
+    n = _page_refs("pages_reserve", page_refs)
+    for what, h in (("kv_lens", kv_lens), ("counts", counts)):
+        _int32("pages_reserve", what, h, (rows,))
+    _int32("pages_reserve", "moves", moves, (rows, 2))
+    _int32("pages_reserve", "info", info, (3,))
+    _lib.call("kh_pages_reserve", page_table.data_ptr(), _row_stride(page_table), kv_lens.data_ptr(), page_refs.data_ptr(),
+              counts.data_ptr(), rows, width, n, page_size, moves.data_ptr(), info.data_ptr())
+
+
+def pages_compact(page_table, page_refs, new_table, new_refs, moves, info) -> None:
+    """Where the live pages go when they move to the front of the pool (kh_pages_compact)."""
+    _page_table("pages_compact", page_table)
+    rows, width = page_table.shape
+    n = _page_refs("pages_compact", page_refs)
+    _int32("pages_compact", "the new page_table", new_table, (rows, width))
+    _int32("pages_compact", "the new page_refs", new_refs, (n,))
+    if len(moves.shape) != 2 or moves.shape[0] < n // 2:
+        raise ValueError(f"pages_compact: moves must be int32 [at least {n // 2}, 2], got {list(moves.shape)}")
+    _int32("pages_compact", "moves", moves, (moves.shape[0], 2))
+    _int32("pages_compact", "info", info, (2,))
+    _lib.call("kh_pages_compact", page_table.data_ptr(), _row_stride(page_table), page_refs.data_ptr(), rows, width, n,
+              new_table.data_ptr(), new_refs.data_ptr(), moves.data_ptr(), moves.shape[0], info.data_ptr())
+
+
+def pages_copy(pages, moves, info) -> None:
+    """Page moves[i, 0] to page moves[i, 1] for i < info[0], in every pool of pages [..., num_pages, Hkv,
+    page size, D] (kh_pages_copy)."""
+    if len(pages.shape) < 4 or not pages.is_contiguous():
+        raise ValueError(f"pages_copy: pages must be contiguous [..., pages, kv heads, page size, head dim], got {list(pages.shape)}")
+    if len(moves.shape) != 2:
+        raise ValueError(f"pages_copy: moves must be int32 [n, 2], got {list(moves.shape)}")
+    _int32("pages_copy", "moves", moves, (moves.shape[0], 2))
+    if info.dtype != INT32 or len(info.shape) != 1 or info.shape[0] < 1 or not info.is_contiguous():
+        raise ValueError(f"pages_copy: info must be an int32 tensor whose first value is the number of moves, got {info.dtype} {list(info.shape)}")
+    sh = pages.shape
+    _lib.call("kh_pages_copy", pages.data_ptr(), math.prod(sh[:-4]), sh[-4], sh[-3] * sh[-2] * sh[-1] * pages.itemsize,
+              moves.data_ptr(), moves.shape[0], info.data_ptr())
+
+
+def beam_select(logits, scores, finished, k: int, eos_token_id, out_scores, out_tokens, out_parents, out_finished) -> None:
+    """The k best continuations of each group of beams (kh_beam_select): logits [groups, beams, vocab],
+    scores float32 [groups, beams], finished int32 [groups, beams] or None; outputs [groups, k]."""
+    if logits.dtype not in (FLOAT32, BFLOAT16):
+        raise TypeError(f"beam_select: logits dtype {logits.dtype} not supported (float32 or bfloat16)")
+    if len(logits.shape) != 3 or not _last_dim_contiguous(logits):
+        raise ValueError(f"beam_select: logits must be [groups, beams, vocab] with contiguous rows, got {list(logits.shape)}")
+    groups, beams, vocab = logits.shape
+    if scores.dtype != FLOAT32 or scores.shape != (groups, beams) or not scores.is_contiguous():
+        raise ValueError(f"beam_select: scores must be contiguous float32 [{groups}, {beams}], got {scores.dtype} {list(scores.shape)}")
+    if (finished is None) != (out_finished is None):
+        raise ValueError("beam_select: finished flags go in and come out together")
+    if finished is not None:
+        _int32("beam_select", "finished", finished, (groups, beams))
+        _int32("beam_select", "the new finished", out_finished, (groups, k))
+        if eos_token_id is None:
+            raise ValueError("beam_select: finished beams need an eos_token_id")
+    if out_scores.dtype != FLOAT32 or out_scores.shape != (groups, k) or not out_scores.is_contiguous():
+        raise ValueError(f"beam_select: the new scores must be contiguous float32 [{groups}, {k}]")
+    _int32("beam_select", "tokens", out_tokens, (groups, k))
+    _int32("beam_select", "parents", out_parents, (groups, k))
+    _lib.call("kh_beam_select", logits.data_ptr(), _lib.i64_array(logits.strides[:2]), scores.data_ptr(),
+              None if finished is None else finished.data_ptr(), groups, beams, vocab, k,
+              -1 if eos_token_id is None else eos_token_id, out_scores.data_ptr(), out_tokens.data_ptr(), out_parents.data_ptr(),
+              None if out_finished is None else out_finished.data_ptr(), logits.kh_dtype)
+
+
 KERNELS = {
+    "paged_attention": paged_attention,
+    "paged_kv_write": paged_kv_write,
+    "pages_fork": pages_fork,
+    "pages_reserve": pages_reserve,
+    "pages_compact": pages_compact,
+    "pages_copy": pages_copy,
+    "beam_select": beam_select,
     "sample": sample,
     "decode_attention_block": decode_attention_block,
     "flash_attention": flash_attention,
