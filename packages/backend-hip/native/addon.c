@@ -706,6 +706,66 @@ FN(gemvSwiglu, 10)
   int64_t k = arg_i64(A, 8); int xdt = arg_int(A, 9);
   CALL(kh_gemv_swiglu(pro, x, nw, (float)eps, w, ldw, h, nh, k, xdt))
 
+/* pagedAttention(q, kPages, vPages, o, pageTable, kvLens, queryStarts | null, tokens, batch, hq, hkv, d, numPages,
+   pageSize, tableWidth, tableStride, strides[10], scale, causal, maxQueryLen, maxKvLen, dtype) */
+FN(pagedAttention, 22)
+  int64_t st[10];
+  void* q = arg_ptr(A, 0); void* kp = arg_ptr(A, 1); void* vp = arg_ptr(A, 2); void* o = arg_ptr(A, 3);
+  void* pt = arg_ptr(A, 4); void* kl = arg_ptr(A, 5); void* qs = arg_ptr(A, 6); int64_t t = arg_i64(A, 7);
+  int64_t b = arg_i64(A, 8); int hq = arg_int(A, 9); int hkv = arg_int(A, 10); int d = arg_int(A, 11);
+  int64_t np = arg_i64(A, 12); int64_t ps = arg_i64(A, 13); int64_t tw = arg_i64(A, 14); int64_t ts = arg_i64(A, 15);
+  arg_list(A, 16, st, 10); double sc = arg_f64(A, 17); int causal = arg_flag(A, 18); int64_t mq = arg_i64(A, 19);
+  int64_t mk = arg_i64(A, 20); int dt = arg_int(A, 21);
+  CALL(kh_paged_attention(q, kp, vp, o, (const int32_t*)pt, (const int32_t*)kl, (const int32_t*)qs, t, b, hq, hkv, d, np, ps,
+                          tw, ts, st, (float)sc, causal, mq, mk, dt))
+/* pagedKvWrite(k, v, kPages, vPages, pageTable, kvLens, queryStarts | null, tokens, batch, hkv, d, numPages, pageSize,
+   tableWidth, tableStride, strides[10], dtype) */
+FN(pagedKvWrite, 17)
+  int64_t st[10];
+  void* k = arg_ptr(A, 0); void* v = arg_ptr(A, 1); void* kp = arg_ptr(A, 2); void* vp = arg_ptr(A, 3);
+  void* pt = arg_ptr(A, 4); void* kl = arg_ptr(A, 5); void* qs = arg_ptr(A, 6); int64_t t = arg_i64(A, 7);
+  int64_t b = arg_i64(A, 8); int hkv = arg_int(A, 9); int d = arg_int(A, 10); int64_t np = arg_i64(A, 11);
+  int64_t ps = arg_i64(A, 12); int64_t tw = arg_i64(A, 13); int64_t ts = arg_i64(A, 14); arg_list(A, 15, st, 10);
+  int dt = arg_int(A, 16);
+  CALL(kh_paged_kv_write(k, v, kp, vp, (const int32_t*)pt, (const int32_t*)kl, (const int32_t*)qs, t, b, hkv, d, np, ps, tw,
+                         ts, st, dt))
+/* pagesFork(pageTable, tableStride, kvLens, pageRefs, parents, rows, tableWidth, numPages, newTable, newLens, newRefs) */
+FN(pagesFork, 11)
+  void* pt = arg_ptr(A, 0); int64_t ts = arg_i64(A, 1); void* kl = arg_ptr(A, 2); void* rf = arg_ptr(A, 3);
+  void* pa = arg_ptr(A, 4); int64_t rows = arg_i64(A, 5); int64_t tw = arg_i64(A, 6); int64_t np = arg_i64(A, 7);
+  void* nt = arg_ptr(A, 8); void* nl = arg_ptr(A, 9); void* nr = arg_ptr(A, 10);
+  CALL(kh_pages_fork((const int32_t*)pt, ts, (const int32_t*)kl, (const int32_t*)rf, (const int32_t*)pa, rows, tw, np,
+                     (int32_t*)nt, (int32_t*)nl, (int32_t*)nr))
+/* pagesReserve(pageTable, tableStride, kvLens, pageRefs, counts, rows, tableWidth, numPages, pageSize, moves, info) */
+FN(pagesReserve, 11)
+  void* pt = arg_ptr(A, 0); int64_t ts = arg_i64(A, 1); void* kl = arg_ptr(A, 2); void* rf = arg_ptr(A, 3);
+  void* ct = arg_ptr(A, 4); int64_t rows = arg_i64(A, 5); int64_t tw = arg_i64(A, 6); int64_t np = arg_i64(A, 7);
+  int64_t ps = arg_i64(A, 8); void* mv = arg_ptr(A, 9); void* in = arg_ptr(A, 10);
+  CALL(kh_pages_reserve((int32_t*)pt, ts, (int32_t*)kl, (int32_t*)rf, (const int32_t*)ct, rows, tw, np, ps, (int32_t*)mv,
+                        (int32_t*)in))
+/* pagesCompact(pageTable, tableStride, pageRefs, rows, tableWidth, numPages, newTable, newRefs, moves, maxMoves, info) */
+FN(pagesCompact, 11)
+  void* pt = arg_ptr(A, 0); int64_t ts = arg_i64(A, 1); void* rf = arg_ptr(A, 2); int64_t rows = arg_i64(A, 3);
+  int64_t tw = arg_i64(A, 4); int64_t np = arg_i64(A, 5); void* nt = arg_ptr(A, 6); void* nr = arg_ptr(A, 7);
+  void* mv = arg_ptr(A, 8); int64_t mm = arg_i64(A, 9); void* in = arg_ptr(A, 10);
+  CALL(kh_pages_compact((const int32_t*)pt, ts, (const int32_t*)rf, rows, tw, np, (int32_t*)nt, (int32_t*)nr, (int32_t*)mv,
+                        mm, (int32_t*)in))
+/* pagesCopy(pages, planes, numPages, pageBytes, moves, maxMoves, info) */
+FN(pagesCopy, 7)
+  void* p = arg_ptr(A, 0); int64_t pl = arg_i64(A, 1); int64_t np = arg_i64(A, 2); int64_t pb = arg_i64(A, 3);
+  void* mv = arg_ptr(A, 4); int64_t mm = arg_i64(A, 5); void* in = arg_ptr(A, 6);
+  CALL(kh_pages_copy(p, pl, np, pb, (const int32_t*)mv, mm, (const int32_t*)in))
+/* beamSelect(logits, strides[2], scores, finished | null, groups, beams, vocab, k, eos, outScores, outTokens, outParents,
+   outFinished | null, dtype) */
+FN(beamSelect, 14)
+  int64_t st[2];
+  void* lg = arg_ptr(A, 0); arg_list(A, 1, st, 2); void* sc = arg_ptr(A, 2); void* fi = arg_ptr(A, 3);
+  int64_t g = arg_i64(A, 4); int64_t b = arg_i64(A, 5); int64_t v = arg_i64(A, 6); int k = arg_int(A, 7);
+  int64_t eos = arg_i64(A, 8); void* os = arg_ptr(A, 9); void* ot = arg_ptr(A, 10); void* op = arg_ptr(A, 11);
+  void* of = arg_ptr(A, 12); int dt = arg_int(A, 13);
+  CALL(kh_beam_select(lg, st, (const float*)sc, (const int32_t*)fi, g, b, v, k, eos, (float*)os, (int32_t*)ot, (int32_t*)op,
+                      (int32_t*)of, dt))
+
 /* ---------------------------------------------------------------- module ----------------------- */
 #define EXPORT(name) {#name, 0, js_##name, 0, 0, 0, napi_enumerable, 0}
 
@@ -722,6 +782,8 @@ static napi_value module_init(napi_env env, napi_value exports) {
       EXPORT(qkNormRope), EXPORT(flashAttention), EXPORT(flashAttentionSplit), EXPORT(flashAttentionMasked), EXPORT(decodeAttention),
       EXPORT(decodeAttentionNoalloc), EXPORT(gemm), EXPORT(gemmEx), EXPORT(gemmSwiglu), EXPORT(gemmQkNormRope), EXPORT(gemmQkNormRopeTable), EXPORT(ropeTable), EXPORT(gemmSplitCount),
       EXPORT(gemmSplitCountFor), EXPORT(gemmSplitkPartials), EXPORT(addRmsNorm), EXPORT(gemvFused), EXPORT(gemvSwiglu),
+      EXPORT(pagedAttention), EXPORT(pagedKvWrite), EXPORT(pagesFork), EXPORT(pagesReserve), EXPORT(pagesCompact), EXPORT(pagesCopy),
+      EXPORT(beamSelect),
   };
   napi_define_properties(env, exports, sizeof(d) / sizeof(d[0]), d);
   napi_value v;

@@ -688,6 +688,149 @@ function decodeAttention(q: HipTensorHandle, kCache: HipTensorHandle, vCache: Hi
                         kCache.shape[2], st, scale, q.kh);
 }
 
+// ---- paged KV cache and beam search ------------------------------------------------------------
+// An int32 operand of `shape` with contiguous data.
+function int32Operand(name: string, what: string, h: HipTensorHandle, shape: number[]): void {
+  if (h.dtype !== 'int32' || h.shape.join() !== shape.join() || !h.isContiguous())
+    throw new Error(`${name}: ${what} must be a contiguous int32 tensor of shape [${shape.join()}]`);
+}
+
+function pageTableOf(name: string, table: HipTensorHandle): number[] {
+  if (table.dtype !== 'int32' || table.shape.length !== 2 || (table.shape[1] > 1 && table.strides[1] !== 1) ||
+      (table.shape[0] > 1 && table.strides[0] < table.shape[1]))
+    throw new Error(`${name}: pageTable must be an int32 tensor [sequences, pages] with contiguous rows`);
+  return [table.shape[0], table.shape[1], table.shape[0] > 1 ? table.strides[0] : table.shape[1]];
+}
+
+// (token, head) strides of [tokens, heads, d] rows, and (page, head, row) strides of page pools.
+function tokenRows(name: string, what: string, h: HipTensorHandle, heads: number, d: number): number[] {
+  if (h.shape.length !== 3 || h.shape[1] !== heads || h.shape[2] !== d || h.strides[2] !== 1)
+    throw new Error(`${name}: ${what} must be [tokens, ${heads}, ${d}] with a contiguous last dim`);
+  return [h.strides[0], h.strides[1]];
+}
+
+function poolStrides(name: string, k: HipTensorHandle, v: HipTensorHandle): number[] {
+  if (k.shape.length !== 4 || v.shape.join() !== k.shape.join() || k.strides[3] !== 1 || v.strides[3] !== 1)
+    throw new Error(`${name}: key and value pages must be [pages, kv heads, page size, head dim] alike`);
+  return k.strides.slice(0, 3).concat(v.strides.slice(0, 3));
+}
+
+function sameFloat(name: string, hs: HipTensorHandle[]): void {
+  for (const h of hs)
+    if (h.dtype === 'int32' || h.dtype !== hs[0].dtype) throw new Error(`${name}: operands must share float32 or bfloat16`);
+}
+
+const NO_LIMIT = 9007199254740991;
+
+// paged_attention(query, keyPages, valuePages, pageTable, kvLens, queryStarts | null, output, scale, isCausal,
+// maxQueryLen?, maxKvLen?): attention of a ragged batch's new tokens over a paged KV cache
+// (kh_paged_attention): query / output [tokens, Hq, D], pools [pages, Hkv, page size, D].
+function pagedAttention(q: HipTensorHandle, kPages: HipTensorHandle, vPages: HipTensorHandle, table: HipTensorHandle,
+                        kvLens: HipTensorHandle, queryStarts: HipTensorHandle | null, out: HipTensorHandle,
+                        scale: number, isCausal: boolean, maxQueryLen?: number, maxKvLen?: number): void {
+  sameFloat('paged_attention', [q, kPages, vPages, out]);
+  const pools = poolStrides('paged_attention', kPages, vPages);
+  const hkv = kPages.shape[1], D = kPages.shape[3], T = q.shape[0], hq = q.shape[1];
+  const qs = tokenRows('paged_attention', 'query', q, hq, D), os = tokenRows('paged_attention', 'output', out, hq, D);
+  if (out.shape[0] !== T) throw new Error('paged_attention: output and query differ in tokens');
+  if (hq % hkv !== 0) throw new Error(`paged_attention: numHeadsQ (${hq}) must be divisible by numHeadsKV (${hkv})`);
+  if (!Number.isFinite(scale)) throw new Error('paged_attention: the scale is not finite');
+  const t = pageTableOf('paged_attention', table);
+  int32Operand('paged_attention', 'kvLens', kvLens, [t[0]]);
+  if (queryStarts !== null) int32Operand('paged_attention', 'queryStarts', queryStarts, [t[0] + 1]);
+  addon.pagedAttention(q.ptr, kPages.ptr, vPages.ptr, out.ptr, table.ptr, kvLens.ptr,
+                       queryStarts === null ? null : queryStarts.ptr, T, t[0], hq, hkv, D, kPages.shape[0], kPages.shape[2],
+                       t[1], t[2], qs.concat(pools, os), scale, isCausal,
+                       maxQueryLen === undefined ? NO_LIMIT : maxQueryLen, maxKvLen === undefined ? NO_LIMIT : maxKvLen,
+                       q.kh);
+}
+
+// paged_kv_write(key, value, keyPages, valuePages, pageTable, kvLens, queryStarts | null): the new tokens' rows
+// [tokens, Hkv, D] into their pages.
+function pagedKvWrite(k: HipTensorHandle, v: HipTensorHandle, kPages: HipTensorHandle, vPages: HipTensorHandle,
+                      table: HipTensorHandle, kvLens: HipTensorHandle, queryStarts: HipTensorHandle | null): void {
+  sameFloat('paged_kv_write', [k, v, kPages, vPages]);
+  const pools = poolStrides('paged_kv_write', kPages, vPages);
+  const hkv = kPages.shape[1], D = kPages.shape[3], T = k.shape[0];
+  const st = tokenRows('paged_kv_write', 'key', k, hkv, D).concat(tokenRows('paged_kv_write', 'value', v, hkv, D));
+  if (v.shape[0] !== T) throw new Error('paged_kv_write: key and value differ in tokens');
+  const t = pageTableOf('paged_kv_write', table);
+  int32Operand('paged_kv_write', 'kvLens', kvLens, [t[0]]);
+  if (queryStarts !== null) int32Operand('paged_kv_write', 'queryStarts', queryStarts, [t[0] + 1]);
+  addon.pagedKvWrite(k.ptr, v.ptr, kPages.ptr, vPages.ptr, table.ptr, kvLens.ptr,
+                     queryStarts === null ? null : queryStarts.ptr, T, t[0], hkv, D, kPages.shape[0], kPages.shape[2], t[1],
+                     t[2], st.concat(pools), k.kh);
+}
+
+// pages_fork(pageTable, kvLens, pageRefs, parents, newTable, newLens, newRefs): rows follow their parents.
+function pagesFork(table: HipTensorHandle, kvLens: HipTensorHandle, refs: HipTensorHandle, parents: HipTensorHandle,
+                   newTable: HipTensorHandle, newLens: HipTensorHandle, newRefs: HipTensorHandle): void {
+  const t = pageTableOf('pages_fork', table);
+  for (const h of [kvLens, parents, newLens]) int32Operand('pages_fork', 'a row operand', h, [t[0]]);
+  int32Operand('pages_fork', 'newTable', newTable, [t[0], t[1]]);
+  int32Operand('pages_fork', 'pageRefs', refs, [refs.numel]);
+  int32Operand('pages_fork', 'newRefs', newRefs, [refs.numel]);
+  addon.pagesFork(table.ptr, t[2], kvLens.ptr, refs.ptr, parents.ptr, t[0], t[1], refs.numel, newTable.ptr, newLens.ptr,
+                  newRefs.ptr);
+}
+
+// pages_reserve(pageTable, kvLens, pageRefs, counts, pageSize, moves, info): rows grow, in place.
+function pagesReserve(table: HipTensorHandle, kvLens: HipTensorHandle, refs: HipTensorHandle, counts: HipTensorHandle,
+                      pageSize: number, moves: HipTensorHandle, info: HipTensorHandle): void {
+  const t = pageTableOf('pages_reserve', table);
+  for (const h of [kvLens, counts]) int32Operand('pages_reserve', 'a row operand', h, [t[0]]);
+  int32Operand('pages_reserve', 'pageRefs', refs, [refs.numel]);
+  int32Operand('pages_reserve', 'moves', moves, [t[0], 2]);
+  int32Operand('pages_reserve', 'info', info, [3]);
+  addon.pagesReserve(table.ptr, t[2], kvLens.ptr, refs.ptr, counts.ptr, t[0], t[1], refs.numel, pageSize, moves.ptr, info.ptr);
+}
+
+// pages_compact(pageTable, pageRefs, newTable, newRefs, moves, info): the live pages to the front of the pool.
+function pagesCompact(table: HipTensorHandle, refs: HipTensorHandle, newTable: HipTensorHandle, newRefs: HipTensorHandle,
+                      moves: HipTensorHandle, info: HipTensorHandle): void {
+  const t = pageTableOf('pages_compact', table);
+  int32Operand('pages_compact', 'pageRefs', refs, [refs.numel]);
+  int32Operand('pages_compact', 'newTable', newTable, [t[0], t[1]]);
+  int32Operand('pages_compact', 'newRefs', newRefs, [refs.numel]);
+  int32Operand('pages_compact', 'moves', moves, [moves.shape[0], 2]);
+  int32Operand('pages_compact', 'info', info, [2]);
+  addon.pagesCompact(table.ptr, t[2], refs.ptr, t[0], t[1], refs.numel, newTable.ptr, newRefs.ptr, moves.ptr, moves.shape[0],
+                     info.ptr);
+}
+
+// pages_copy(pages, moves, info): page moves[i][0] to page moves[i][1] for i < info[0], in every pool of pages
+// [..., num_pages, Hkv, page size, D].
+function pagesCopy(pages: HipTensorHandle, moves: HipTensorHandle, info: HipTensorHandle): void {
+  const n = pages.shape.length;
+  if (n < 4 || !pages.isContiguous()) throw new Error('pages_copy: contiguous pages [..., pages, kv heads, page size, head dim] expected');
+  int32Operand('pages_copy', 'moves', moves, [moves.shape[0], 2]);
+  if (info.numel < 1) throw new Error('pages_copy: info must hold the number of moves');
+  int32Operand('pages_copy', 'info', info, [info.numel]);
+  const planes = pages.shape.slice(0, n - 4).reduce((a: number, b: number): number => a * b, 1);
+  const page = pages.shape[n - 3] * pages.shape[n - 2] * pages.shape[n - 1] * (pages.dtype === 'bfloat16' ? 2 : 4);
+  addon.pagesCopy(pages.ptr, planes, pages.shape[n - 4], page, moves.ptr, moves.shape[0], info.ptr);
+}
+
+// beam_select(logits, scores, finished | null, k, eosTokenId, outScores, outTokens, outParents, outFinished | null): the k
+// best continuations of each group of beams over beams x vocabulary (kh_beam_select).
+function beamSelect(logits: HipTensorHandle, scores: HipTensorHandle, finished: HipTensorHandle | null, k: number,
+                    eosTokenId: number, outScores: HipTensorHandle, outTokens: HipTensorHandle,
+                    outParents: HipTensorHandle, outFinished: HipTensorHandle | null): void {
+  if (logits.dtype === 'int32' || logits.shape.length !== 3 || logits.strides[2] !== 1)
+    throw new Error('beam_select: float logits [groups, beams, vocab] with contiguous rows expected');
+  const g = logits.shape[0], b = logits.shape[1];
+  for (const h of [scores, outScores])
+    if (h.dtype !== 'float32' || h.shape.join() !== [g, h === scores ? b : k].join() || !h.isContiguous())
+      throw new Error('beam_select: contiguous float32 scores [groups, beams] and [groups, k] expected');
+  int32Operand('beam_select', 'tokens', outTokens, [g, k]);
+  int32Operand('beam_select', 'parents', outParents, [g, k]);
+  if (finished !== null) int32Operand('beam_select', 'finished', finished, [g, b]);
+  if (outFinished !== null) int32Operand('beam_select', 'the new finished', outFinished, [g, k]);
+  addon.beamSelect(logits.ptr, logits.strides.slice(0, 2), scores.ptr, finished === null ? null : finished.ptr, g, b,
+                   logits.shape[2], k, eosTokenId, outScores.ptr, outTokens.ptr, outParents.ptr,
+                   outFinished === null ? null : outFinished.ptr, logits.kh);
+}
+
 // rms_norm_rope(q, k, params): per-head RMSNorm with q_norm / k_norm weights and RoPE at int32
 // positions, for q [B, S, Hq, D] and k [B, S, Hkv, D] (gqa.ts:279-309 then rope.ts:590-630), written
 // heads-first ([B, H, S, D]).  params: qWeight, kWeight, invFreq (float32 [D/2]), positions (int32
@@ -1056,6 +1199,13 @@ export function registerHipKernels(reg: SimpleOperatorRegistry): void {
     [sc.start === undefined ? 0 : Number(sc.start), sc.step === undefined ? 1 : Number(sc.step)]));
   reg.register('argmax', argmaxKernel);
   reg.register('decode_attention', decodeAttention);
+  reg.register('paged_attention', pagedAttention);
+  reg.register('paged_kv_write', pagedKvWrite);
+  reg.register('pages_fork', pagesFork);
+  reg.register('pages_reserve', pagesReserve);
+  reg.register('pages_compact', pagesCompact);
+  reg.register('pages_copy', pagesCopy);
+  reg.register('beam_select', beamSelect);
   reg.register('rms_norm_rope', rmsNormRope);
   reg.register('silu_mul', siluMul);
   reg.register('index_select', indexSelect);
