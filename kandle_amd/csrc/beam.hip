@@ -13,8 +13,9 @@ namespace {
 
 constexpr int kMaxK = 64;
 constexpr int kMaxBeams = 64;
+constexpr float kLog2e = 1.4426950408889634f;
 
-// Order-preserving bits of a logit (-0 as +0), 1 at least: 0 stands for no candidate.
+// Order-preserving bits (-0 as +0), above 0 for every number: 0 stands for no candidate.
 __device__ __forceinline__ uint32_t order_bits(float x) {
   const uint32_t b = __float_as_uint(x == 0.f ? 0.f : x);
   return (b & 0x80000000u) ? ~b : (b | 0x80000000u);
@@ -22,148 +23,243 @@ __device__ __forceinline__ uint32_t order_bits(float x) {
 __device__ __forceinline__ float order_value(uint32_t u) {
   return __uint_as_float((u & 0x80000000u) ? (u & 0x7fffffffu) : ~u);
 }
-__device__ __forceinline__ uint64_t order_key(float x, int id) {
-  return ((uint64_t)order_bits(x) << 32) | (uint64_t)(0xffffffffu - (uint32_t)id);
+__device__ __forceinline__ uint64_t order_bits(double x) {
+  const uint64_t b = (uint64_t)__double_as_longlong(x == 0.0 ? 0.0 : x);
+  return (b >> 63) ? ~b : (b | 0x8000000000000000ull);
+}
+__device__ __forceinline__ double order_value(uint64_t u) {
+  return __longlong_as_double((long long)((u >> 63) ? (u & 0x7fffffffffffffffull) : ~u));
 }
 __device__ __forceinline__ float no_nan(float x) { return x != x ? -INFINITY : x; }
 
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+// A candidate: the larger `hi` first, then the lower `at`.  hi 0: none.  Logits hold their order bits in the
+// upper half of hi; the merge holds those of a float64 score.
+struct Cand {
+  uint64_t hi;
+  int64_t at;
+};
+__device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.hi > b.hi || (a.hi == b.hi && a.at < b.at); }
+
+// The k best of a wave's candidates, N per lane in registers, in order to out[0 .. k) (LDS; none behind the
+// last); `room` is the wave's own LDS for kRoom candidates.
+//
+// The k-th largest of the lanes' maxima (of hi's upper word) is at most the k-th largest candidate, so
+// nothing below it is wanted; a handful above it are left, which are ranked by counting.  It is found bit
+// by bit with ballots.  Where more than kRoom are left (many equal values), k rounds of a wave-wide
+// maximum do the same.
+constexpr int kRoom = 128;
+template <int N>
+__device__ __forceinline__ void wave_best(Cand (&c)[N], int k, Cand* room, Cand* out) {
+  const int lane = threadIdx.x & 63;
+  uint32_t top = 0;
 #pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const uint64_t u = __shfl_xor(v, o, 64);
-    v = u > v ? u : v;
+  for (int i = 0; i < N; ++i) top = max(top, (uint32_t)(c[i].hi >> 32));
+  uint32_t floor = 0;
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t t = floor | (1u << b);
+    const int n = __popcll(__ballot(top >= t));
+    if (n >= k) floor = t;
+    if (n == k) break;
   }
-  return v;
+  int count = 0;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const bool keep = c[i].hi != 0 && (uint32_t)(c[i].hi >> 32) >= floor;
+    const uint64_t who = __ballot(keep);
+    if (who != 0) {
+      const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+      if (keep && at < kRoom) room[at] = c[i];
+      count += __popcll(who);
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
+  if (count <= kRoom) {
+    for (int j = lane; j < k; j += 64) out[j] = Cand{0, 0};
+    __builtin_amdgcn_wave_barrier();
+    for (int j = lane; j < count; j += 64) {
+      const Cand mine = room[j];
+      int rank = 0;
+      for (int i = 0; i < count; ++i) rank += before(room[i], mine);
+      if (rank < k) out[rank] = mine;
+    }
+  } else {
+    for (int j = 0; j < k; ++j) {
+      Cand best{0, 0};
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c[i].hi != 0 && (best.hi == 0 || before(c[i], best))) best = c[i];
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        const Cand u{__shfl_xor(best.hi, o, 64), __shfl_xor(best.at, o, 64)};
+        if (u.hi != 0 && (best.hi == 0 || before(u, best))) best = u;
+      }
+#pragma unroll
+      for (int i = 0; i < N; ++i)
+        if (c[i].hi == best.hi && c[i].at == best.at) c[i].hi = 0;
+      if (lane == 0) out[j] = best;
+    }
+  }
+  __builtin_amdgcn_wave_barrier();
 }
 
-// A wave per run of 1024 logits of a row: their maximum, their sum of exponentials relative to it, and the
-// keys of the k largest in order (0 behind the last).
-constexpr int kRun = 1024, kPer = kRun / 64;
+// A workgroup takes a run of 8192 logits of one row, 32 per lane in registers: their maximum, the sum of
+// exponentials relative to it, and the k largest in order.  Rows may start anywhere: the lanes' 16-byte loads
+// lie on the 16-byte grid of the memory, and those that cross a row's ends are made value by value.
+constexpr int kPer = 32, kRunWaves = 4, kRun = kPer * 64 * kRunWaves;
 template <typename T>
-__global__ __launch_bounds__(64) void beam_runs_kernel(const T* __restrict__ logits, int64_t sg, int64_t sb, int beams,
-                                                       int vocab, const int32_t* __restrict__ finished, int k, int runs,
-                                                       float2* __restrict__ sums, uint64_t* __restrict__ keys) {
-  const int row = blockIdx.y, run = blockIdx.x, lane = threadIdx.x;
+__global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __restrict__ logits, int64_t sg, int64_t sb,
+                                                                   int beams, int vocab,
+                                                                   const int32_t* __restrict__ finished, int k, int runs,
+                                                                   float2* __restrict__ sums, uint64_t* __restrict__ keys) {
+  constexpr int E = 16 / sizeof(T);
+  __shared__ Cand room[kRunWaves][kRoom];
+  __shared__ Cand best[kRunWaves * kMaxK];
+  __shared__ float2 part[kRunWaves];
+  const int row = blockIdx.y, run = blockIdx.x, lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (finished && finished[row] != 0) return;
-  const T* x = logits + (row / beams) * sg + (row % beams) * sb;
-  uint64_t key[kPer];
-  float v[kPer], m = -INFINITY;
+  const T* x = logits + (int64_t)(row / beams) * sg + (int64_t)(row % beams) * sb;
+  const int shift = (int)(((uintptr_t)x & 15) / sizeof(T));
+  const int64_t start = (int64_t)run * kRun + w * (kRun / kRunWaves) + lane * E - shift;
+  float v[kPer];
+#pragma unroll
+  for (int j = 0; j < kPer / E; ++j) {
+    const int64_t id = start + j * 64 * E;
+    if (id >= 0 && id + E <= vocab) {
+      const uint4 u = *reinterpret_cast<const uint4*>(x + id);
+      if constexpr (E == 4) {
+        v[4 * j] = __uint_as_float(u.x);
+        v[4 * j + 1] = __uint_as_float(u.y);
+        v[4 * j + 2] = __uint_as_float(u.z);
+        v[4 * j + 3] = __uint_as_float(u.w);
+      } else {
+        float f[8];
+        unpack_bf16x8(u, f);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[8 * j + e] = f[e];
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[E * j + e] = id + e >= 0 && id + e < vocab ? Elem<T>::load(x, id + e) : -INFINITY;
+    }
+  }
+  float m = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int id = run * kRun + i * 64 + lane;
-    v[i] = id < vocab ? no_nan(Elem<T>::load(x, id)) : -INFINITY;
-    key[i] = id < vocab ? order_key(v[i], id) : 0;
+    v[i] = no_nan(v[i]);
     m = fmaxf(m, v[i]);
   }
   m = wave_max(m);
   float s = 0.f;
   if (m > -INFINITY)
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) s += __expf(v[i] - m);
+    for (int i = 0; i < kPer; ++i) s += fast_exp2((v[i] - m) * kLog2e);
   s = wave_sum(s);
-  if (lane == 0) sums[(int64_t)row * runs + run] = make_float2(m, s);
-  for (int j = 0; j < k; ++j) {
-    uint64_t best = 0;
+  Cand c[kPer];
 #pragma unroll
-    for (int i = 0; i < kPer; ++i) best = key[i] > best ? key[i] : best;
-    best = wave_max_u64(best);
+  for (int i = 0; i < kPer; ++i) {
+    const int64_t id = start + (int64_t)(i / E) * 64 * E + i % E;
+    c[i] = Cand{id >= 0 && id < vocab ? (uint64_t)order_bits(v[i]) << 32 : 0, id};
+  }
+  wave_best<kPer>(c, k, room[w], best + w * k);
+  if (lane == 0) part[w] = make_float2(m, s);
+  __syncthreads();
+  const int64_t o = (int64_t)row * runs + run;
+  if (threadIdx.x == 0) {
+    float mm = part[0].x, ss = 0.f;
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      if (key[i] == best) key[i] = 0;
-    if (lane == 0) keys[((int64_t)row * runs + run) * k + j] = best;
+    for (int i = 1; i < kRunWaves; ++i) mm = fmaxf(mm, part[i].x);
+#pragma unroll
+    for (int i = 0; i < kRunWaves; ++i)
+      if (part[i].x > -INFINITY) ss += part[i].y * fast_exp2((part[i].x - mm) * kLog2e);
+    sums[o] = make_float2(mm, ss);
+  }
+  // the waves' best joined: each is ranked among all
+  for (int j = threadIdx.x; j < kRunWaves * k; j += kRunWaves * 64) {
+    const Cand mine = best[j];
+    int rank = 0;
+    for (int i = 0; i < kRunWaves * k; ++i) {
+      const Cand u = best[i];
+      rank += before(u, mine) || (u.hi == 0 && mine.hi == 0 && i < j);
+    }
+    if (rank < k) keys[o * k + rank] = mine.hi == 0 ? 0 : mine.hi | (uint32_t)mine.at;
   }
 }
 
-// A candidate of the last selection: its score and its place beam * vocab + token.
-struct Best {
-  double score;
-  int64_t at;  // -1: none
-};
-__device__ __forceinline__ bool better(const Best& a, const Best& b) {
-  if (a.at < 0 || b.at < 0) return b.at < 0 && a.at >= 0;
-  return a.score > b.score || (a.score == b.score && a.at < b.at);
-}
-
-// A workgroup per group: the sums of its beams, then k rounds of the best candidate left.
-__global__ __launch_bounds__(256) void beam_merge_kernel(const float2* __restrict__ sums, const uint64_t* __restrict__ keys,
-                                                         const float* __restrict__ scores,
-                                                         const int32_t* __restrict__ finished, int beams, int vocab, int k,
-                                                         int runs, int eos, float* __restrict__ out_scores,
-                                                         int32_t* __restrict__ out_tokens, int32_t* __restrict__ out_parents,
-                                                         int32_t* __restrict__ out_finished) {
+// A workgroup per group: the sums of its beams, then the k best of the runs' candidates, scored in float64.
+constexpr int kMergeWaves = 16, kSlots = 2;
+__global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
+    const float2* __restrict__ sums, const uint64_t* __restrict__ keys, const float* __restrict__ scores,
+    const int32_t* __restrict__ finished, int beams, int vocab, int k, int runs, int eos, float* __restrict__ out_scores,
+    int32_t* __restrict__ out_tokens, int32_t* __restrict__ out_parents, int32_t* __restrict__ out_finished) {
   __shared__ double base[kMaxBeams];  // scores[beam] - log sum exp, or NaN where all the beam's scores are -inf
-  __shared__ double best_score[4];
-  __shared__ int64_t best_at[4];
-  const int g = blockIdx.x, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  for (int b = w; b < beams; b += 4) {
+  __shared__ int done[kMaxBeams];
+  __shared__ Cand room[kMergeWaves][kRoom];
+  __shared__ Cand best[kMergeWaves * kMaxK];
+  const int g = blockIdx.x, lane = threadIdx.x & 63;
+  const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  for (int b = w; b < beams; b += kMergeWaves) {
     const int row = g * beams + b;
     const double sc = (double)scores[row];
-    if (finished && finished[row] != 0) {
-      if (lane == 0) base[b] = sc;
-      continue;
-    }
-    float m = -INFINITY;
-    for (int r = lane; r < runs; r += 64) m = fmaxf(m, sums[(int64_t)row * runs + r].x);
-    m = wave_max(m);
-    double s = 0.0;
-    for (int r = lane; r < runs; r += 64) {
-      const float2 ms = sums[(int64_t)row * runs + r];
-      if (ms.x > -INFINITY) s += (double)ms.y * exp((double)ms.x - (double)m);
-    }
+    const bool fin = finished && finished[row] != 0;
+    double v = sc;
+    if (!fin) {
+      float m = -INFINITY;
+      for (int r = lane; r < runs; r += 64) m = fmaxf(m, sums[(int64_t)row * runs + r].x);
+      m = wave_max(m);
+      double s = 0.0;
+      for (int r = lane; r < runs; r += 64) {
+        const float2 ms = sums[(int64_t)row * runs + r];
+        if (ms.x > -INFINITY) s += (double)ms.y * exp((double)ms.x - (double)m);
+      }
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+      for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+      v = sc - ((double)m + log(s));
+    }
     if (lane == 0) {
-      const double v = sc - ((double)m + log(s));
       base[b] = v == v && v > -INFINITY && v < INFINITY ? v : __builtin_nan("");
+      done[b] = fin;
     }
   }
   __syncthreads();
   const int per = runs * k;
-  Best last{INFINITY, -1};  // the one chosen last: the next one is the best behind it
-  for (int j = 0; j < k; ++j) {
-    Best mine{-INFINITY, -1};
-    for (int64_t i = threadIdx.x; i < (int64_t)beams * per; i += 256) {
-      const int b = (int)(i / per), c = (int)(i - (int64_t)b * per);
-      const bool done = finished && finished[g * beams + b] != 0;
-      Best x{-INFINITY, -1};
-      if (done) {
-        if (c == 0) x = Best{base[b] == base[b] ? base[b] : -INFINITY, (int64_t)b * vocab + eos};
-      } else if (base[b] != base[b]) {
-        if (c < k && c < vocab) x = Best{-INFINITY, (int64_t)b * vocab + c};
-      } else {
-        const uint64_t key = keys[(int64_t)(g * beams + b) * per + c];
-        if (key != 0)
-          x = Best{(double)order_value((uint32_t)(key >> 32)) + base[b],
-                   (int64_t)b * vocab + (int64_t)(0xffffffffu - (uint32_t)key)};
+  const int64_t all = (int64_t)beams * per;
+  Cand* mine = best + w * k;
+  for (int j = lane; j < k; j += 64) mine[j] = Cand{0, 0};
+  for (int64_t i0 = 0; i0 < all; i0 += kMergeWaves * 64 * kSlots) {
+    Cand c[kSlots + 1];
+#pragma unroll
+    for (int i = 0; i < kSlots; ++i) {
+      const int64_t at = i0 + (int64_t)(w * kSlots + i) * 64 + lane;
+      c[i] = Cand{0, 0};
+      if (at < all) {
+        const int b = (int)(at / per), n = (int)(at - (int64_t)b * per);
+        if (done[b]) {
+          if (n == 0) c[i] = Cand{order_bits(base[b] == base[b] ? base[b] : -(double)INFINITY), (int64_t)b * vocab + eos};
+        } else if (base[b] != base[b]) {
+          if (n < k && n < vocab) c[i] = Cand{order_bits(-(double)INFINITY), (int64_t)b * vocab + n};
+        } else {
+          const uint64_t key = keys[(int64_t)(g * beams + b) * per + n];
+          if (key != 0)
+            c[i] = Cand{order_bits((double)order_value((uint32_t)(key >> 32)) + base[b]), (int64_t)b * vocab + (uint32_t)key};
+        }
       }
-      if (x.at >= 0 && (last.at < 0 || better(last, x)) && better(x, mine)) mine = x;
     }
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-      const Best u{__shfl_xor(mine.score, o, 64), __shfl_xor(mine.at, o, 64)};
-      if (better(u, mine)) mine = u;
-    }
-    __syncthreads();
-    if (lane == 0) {
-      best_score[w] = mine.score;
-      best_at[w] = mine.at;
-    }
-    __syncthreads();
-    last = Best{best_score[0], best_at[0]};
-#pragma unroll
-    for (int i = 1; i < 4; ++i) {
-      const Best u{best_score[i], best_at[i]};
-      if (better(u, last)) last = u;
-    }
-    if (threadIdx.x == 0) {
-      const int b = last.at < 0 ? 0 : (int)(last.at / vocab), t = last.at < 0 ? 0 : (int)(last.at - (int64_t)b * vocab);
-      const int o = g * k + j;
-      out_scores[o] = (float)last.score;
-      out_tokens[o] = t;
-      out_parents[o] = b;
-      if (out_finished) out_finished[o] = (finished[g * beams + b] != 0 || t == eos) ? 1 : 0;
-    }
-    if (last.at < 0) break;
+    c[kSlots] = lane < k ? mine[lane] : Cand{0, 0};  // the best so far
+    wave_best<kSlots + 1>(c, k, room[w], mine);
+  }
+  __syncthreads();
+  for (int j = threadIdx.x; j < kMergeWaves * k; j += kMergeWaves * 64) {
+    const Cand u = best[j];
+    if (u.hi == 0) continue;
+    int rank = 0;
+    for (int i = 0; i < kMergeWaves * k; ++i) rank += before(best[i], u);
+    if (rank >= k) continue;
+    const int b = (int)(u.at / vocab), t = (int)(u.at - (int64_t)b * vocab), o = g * k + rank;
+    out_scores[o] = (float)order_value(u.hi);
+    out_tokens[o] = t;
+    out_parents[o] = b;
+    if (out_finished) out_finished[o] = (done[b] || t == eos) ? 1 : 0;
   }
 }
 
@@ -188,7 +284,8 @@ int kh_beam_select(const void* logits, const int64_t* strides, const float* scor
   if (groups == 0) return KH_OK;
   KH_REQUIRE(logits && strides && scores && out_scores && out_tokens && out_parents, "kh_beam_select: null pointer");
   const int64_t rows = groups * beams;
-  const int runs = (int)((vocab + kRun - 1) / kRun);
+  const int shift = (dtype == KH_BF16 ? 8 : 4) - 1;  // a row may start this far inside a 16-byte block
+  const int runs = (int)((vocab + shift + kRun - 1) / kRun);
   const size_t sum_bytes = ((size_t)rows * runs * sizeof(float2) + 255) / 256 * 256;
   uint8_t* scratch = (uint8_t*)scratch_alloc(sum_bytes + (size_t)rows * runs * k * 8);
   if (scratch == nullptr) return KH_ERR_OOM;
@@ -196,14 +293,14 @@ int kh_beam_select(const void* logits, const int64_t* strides, const float* scor
   uint64_t* keys = (uint64_t*)(scratch + sum_bytes);
   const dim3 grid((unsigned)runs, (unsigned)rows);
   if (dtype == KH_BF16)
-    beam_runs_kernel<uint16_t><<<grid, 64, 0, stream()>>>((const uint16_t*)logits, strides[0], strides[1], (int)beams,
+    beam_runs_kernel<uint16_t><<<grid, kRunWaves * 64, 0, stream()>>>((const uint16_t*)logits, strides[0], strides[1], (int)beams,
                                                           (int)vocab, finished, k, runs, sums, keys);
   else
-    beam_runs_kernel<float><<<grid, 64, 0, stream()>>>((const float*)logits, strides[0], strides[1], (int)beams, (int)vocab,
+    beam_runs_kernel<float><<<grid, kRunWaves * 64, 0, stream()>>>((const float*)logits, strides[0], strides[1], (int)beams, (int)vocab,
                                                        finished, k, runs, sums, keys);
   hipError_t e = hipGetLastError();
   if (e == hipSuccess) {
-    beam_merge_kernel<<<(unsigned)groups, 256, 0, stream()>>>(sums, keys, scores, finished, (int)beams, (int)vocab, k, runs,
+    beam_merge_kernel<<<(unsigned)groups, kMergeWaves * 64, 0, stream()>>>(sums, keys, scores, finished, (int)beams, (int)vocab, k, runs,
                                                               (int)eos, out_scores, out_tokens, out_parents, out_finished);
     e = hipGetLastError();
   }
