@@ -42,6 +42,102 @@ struct PagedBatch {
   }
 };
 
+struct PagedStrides {
+  int64_t qt, qh, kp, kh, kr, vp, vh, vr, ot, oh;
+};
+
+// The (sequence, tile) of workgroup column x of a grid over tiles of `rows` packed rows: sequence b has
+// ceil(min(n_b, max_new) * G / rows) tiles, none unless above < min(n_b, max_new) * G <= upto.  Every wave of the
+// workgroup computes it for itself; b = -1: nothing to do.
+struct Tile {
+  int b = -1, row0 = 0, rows = 0;  // first packed row, packed rows of the sequence
+  int t0 = 0, n = 0, len = 0;      // first token, new tokens, cached rows
+};
+__device__ __forceinline__ Tile find_tile(const PagedBatch& pb, int x, int G, int rows, int max_new, int above, int upto) {
+  Tile t;
+  int at = x;
+  if (pb.starts == nullptr) {
+    const int per = (G + rows - 1) / rows;
+    t.b = x / per;
+    at = x - t.b * per;
+    if (t.b >= pb.batch) t.b = -1;
+  } else {
+    const int lane = threadIdx.x & 63;
+    for (int b0 = 0; b0 < pb.batch; b0 += 64) {
+      const int b = b0 + lane;
+      const int n = b < pb.batch ? min(pb.count(b), max_new) : 0;
+      const int tiles = n * G > above && n * G <= upto ? (n * G + rows - 1) / rows : 0;
+      int inc = tiles;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(inc, o, 64);
+        if (lane >= o) inc += u;
+      }
+      const int all = __shfl(inc, 63, 64);
+      if (at < all) {
+        const int who = __ffsll((unsigned long long)__ballot(inc > at)) - 1;
+        at -= __shfl(inc - tiles, who, 64);
+        t.b = b0 + who;
+        break;
+      }
+      at -= all;
+    }
+  }
+  t.b = __builtin_amdgcn_readfirstlane(t.b);
+  if (t.b < 0) return t;
+  at = __builtin_amdgcn_readfirstlane(at);
+  t.t0 = pb.first(t.b);
+  t.n = pb.count(t.b);
+  t.len = pb.len(t.b);
+  t.row0 = at * rows;
+  t.rows = min(t.n, max_new) * G;
+  if (t.row0 < 0 || t.row0 >= t.rows) t.b = -1;  // (starts that overlap can claim more tiles than there are)
+  return t;
+}
+
+// Keys that token j of the tile's sequence sees: those below the result (holes apart).
+__device__ __forceinline__ int seen_by(const Tile& t, int j, int causal, int max_len) {
+  return min(max_len, causal ? max(0, t.len - t.n + j + 1) : t.len);
+}
+
+// Partials of chunk s of packed row x of sequence b: its (token, head) pair's row in `part`, chunk s.
+// O relative to m (not divided by l), then m (raw units) and l.
+template <int D>
+__device__ __forceinline__ float* part_o(float* part, int64_t row, int chunks, int s) {
+  return part + (row * chunks + s) * D;
+}
+template <int D>
+__device__ __forceinline__ float2* part_ml(float* part, int64_t all_rows, int chunks, int64_t row) {
+  return reinterpret_cast<float2*>(part + all_rows * chunks * D) + row * chunks;
+}
+template <int D>
+__device__ __forceinline__ const float2* part_ml(const float* part, int64_t all_rows, int chunks, int64_t row) {
+  return reinterpret_cast<const float2*>(part + all_rows * chunks * D) + row * chunks;
+}
+
+// One call of kh_paged_attention.
+struct PagedCall {
+  const void *q, *k, *v;
+  void* o;
+  PagedBatch pb;
+  int hq, hkv, G;
+  PagedStrides st;
+  float c2, sign;  // |scale| log2 e, and the scale's sign, which goes to the queries; scale 0: 1 and queries of 0
+  int causal, max_new;
+};
+
+// Workgroup columns that cover every tile of `rows` packed rows.
+inline int64_t tiles_of(const PagedCall& c, int rows) {
+  const int64_t per = ((int64_t)c.max_new * c.G + rows - 1) / rows;
+  const int64_t all = (int64_t)c.pb.tokens * c.G / rows + c.pb.batch;
+  return c.pb.starts == nullptr || per * c.pb.batch < all ? per * c.pb.batch : all;
+}
+
+// paged_tiles.hip: the call's sequences of more than min_rows packed rows, bfloat16, d 64 or 128, in tiles of
+// 32 `waves` (4 or 8) rows; chunks of `chunk` keys (a multiple of 128), with partials unless there is one.
+void launch_paged_tiles(const PagedCall& c, int d, int waves, int min_rows, int64_t tiles, int chunk, int chunks,
+                        float* part);
+
 inline int log2_of(int64_t v) {
   int n = 0;
   while ((int64_t(1) << n) < v) ++n;

@@ -10,72 +10,15 @@
 // Work is split over tiles of packed rows and over chunks of `chunk` keys; where a tile's keys make more
 // than one chunk, each chunk leaves (O, m, l) partials and paged_merge_kernel joins them in chunk order, so
 // a result does not depend on timing.
+#include <cstdlib>
 #include <type_traits>
 
+#include "flash_tiles.h"
 #include "paged.h"
 
 using namespace kh;
 
 namespace {
-
-constexpr float kLog2e = 1.4426950408889634f;
-constexpr float kSumMax = 4096.f;  // a lane's sum of P above this raises the reference maximum
-
-struct PagedStrides {
-  int64_t qt, qh, kp, kh, kr, vp, vh, vr, ot, oh;
-};
-
-// The (sequence, tile) of workgroup column x of a grid over tiles of `rows` packed rows: sequence b has
-// ceil(min(n_b, max_new) * G / rows) tiles.  Every wave of the workgroup computes it for itself.
-struct Tile {
-  int b = -1, row0 = 0, rows = 0;  // first packed row, packed rows of the sequence
-  int t0 = 0, n = 0, len = 0;      // first token, new tokens, cached rows
-};
-__device__ __forceinline__ Tile find_tile(const PagedBatch& pb, int x, int G, int rows, int max_new) {
-  Tile t;
-  int at = x;
-  if (pb.starts == nullptr) {
-    const int per = (G + rows - 1) / rows;
-    t.b = x / per;
-    at = x - t.b * per;
-    if (t.b >= pb.batch) t.b = -1;
-  } else {
-    const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < pb.batch; b0 += 64) {
-      const int b = b0 + lane;
-      const int n = b < pb.batch ? min(pb.count(b), max_new) : 0;
-      const int tiles = (int)(((int64_t)n * G + rows - 1) / rows);
-      int inc = tiles;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(inc, o, 64);
-        if (lane >= o) inc += u;
-      }
-      const int all = __shfl(inc, 63, 64);
-      if (at < all) {
-        const int who = __ffsll((unsigned long long)__ballot(inc > at)) - 1;
-        at -= __shfl(inc - tiles, who, 64);
-        t.b = b0 + who;
-        break;
-      }
-      at -= all;
-    }
-  }
-  t.b = __builtin_amdgcn_readfirstlane(t.b);
-  if (t.b < 0) return t;
-  at = __builtin_amdgcn_readfirstlane(at);
-  t.t0 = pb.first(t.b);
-  t.n = pb.count(t.b);
-  t.len = pb.len(t.b);
-  t.row0 = at * rows;
-  t.rows = min(t.n, max_new) * G;
-  return t;
-}
-
-// Keys that token j of the tile's sequence sees: those below the result (holes apart).
-__device__ __forceinline__ int seen_by(const Tile& t, int j, int causal, int max_len) {
-  return min(max_len, causal ? max(0, t.len - t.n + j + 1) : t.len);
-}
 
 // ---- few rows: K and V straight from the pages into MFMA operands --------------------------------
 //
@@ -110,27 +53,33 @@ struct RowOps<uint16_t, D> {
   struct Q {
     bf16x8 v[NK];
   };
-  static __device__ __forceinline__ void load_q(Q& q, const uint16_t* row, int lq, bool there, float sign) {
-    const uint32_t flip = sign < 0.f ? 0x80008000u : 0u;
+  // A query row, and the row times sign (0: zeros whatever it holds).
+  static __device__ __forceinline__ void load_q(Q& q, const uint16_t* row, int lq) {
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+      q.v[c] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(row + 32 * c + 8 * lq));
+  }
+  static __device__ __forceinline__ void sign_q(Q& q, float sign) {
+    const uint32_t flip = sign < 0.f ? 0x80008000u : 0u, keep = sign != 0.f ? ~0u : 0u;
 #pragma unroll
     for (int c = 0; c < NK; ++c) {
-      uint4 u = there ? *reinterpret_cast<const uint4*>(row + 32 * c + 8 * lq) : make_uint4(0, 0, 0, 0);
-      u.x ^= flip;
-      u.y ^= flip;
-      u.z ^= flip;
-      u.w ^= flip;
+      uint4 u = __builtin_bit_cast(uint4, q.v[c]);
+      u.x = (u.x ^ flip) & keep;
+      u.y = (u.y ^ flip) & keep;
+      u.z = (u.z ^ flip) & keep;
+      u.w = (u.w ^ flip) & keep;
       q.v[c] = __builtin_bit_cast(bf16x8, u);
     }
   }
   static __device__ __forceinline__ void load_k(K& k, __amdgpu_buffer_rsrc_t r, uint32_t off, int lq) {
 #pragma unroll
-    for (int c = 0; c < NK; ++c) k.v[c] = buf_load16_nt(r, off + 64 * c + 16 * lq);
+    for (int c = 0; c < NK; ++c) k.v[c] = buf_load16(r, off + 64 * c + 16 * lq);
   }
   static __device__ __forceinline__ void load_v(VRow& v, __amdgpu_buffer_rsrc_t r, uint32_t off) {
     if constexpr (EPL == 8)
-      v = buf_load16_nt(r, off);
+      v = buf_load16(r, off);
     else
-      v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 2));
+      v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
   }
   static __device__ __forceinline__ f32x4 qk(const K& k, const Q& q, f32x4 s) {
 #pragma unroll
@@ -216,20 +165,23 @@ struct RowOps<float, D> {
   struct Q {
     f32x4 v[NK];
   };
-  static __device__ __forceinline__ void load_q(Q& q, const float* row, int lq, bool there, float sign) {
+  static __device__ __forceinline__ void load_q(Q& q, const float* row, int lq) {
 #pragma unroll
-    for (int c = 0; c < NK; ++c) {
-      const f32x4 z = {0.f, 0.f, 0.f, 0.f};
-      q.v[c] = there ? *reinterpret_cast<const f32x4*>(row + 16 * c + 4 * lq) * sign : z;
-    }
+    for (int c = 0; c < NK; ++c) q.v[c] = *reinterpret_cast<const f32x4*>(row + 16 * c + 4 * lq);
+  }
+  static __device__ __forceinline__ void sign_q(Q& q, float sign) {
+#pragma unroll
+    for (int c = 0; c < NK; ++c)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) q.v[c][i] = sign == 0.f ? 0.f : q.v[c][i] * sign;
   }
   static __device__ __forceinline__ void load_k(K& k, __amdgpu_buffer_rsrc_t r, uint32_t off, int lq) {
 #pragma unroll
-    for (int c = 0; c < NK; ++c) k.v[c] = __builtin_bit_cast(f32x4, buf_load16_nt(r, off + 64 * c + 16 * lq));
+    for (int c = 0; c < NK; ++c) k.v[c] = __builtin_bit_cast(f32x4, buf_load16(r, off + 64 * c + 16 * lq));
   }
   static __device__ __forceinline__ void load_v(VRow& v, __amdgpu_buffer_rsrc_t r, uint32_t off) {
 #pragma unroll
-    for (int i = 0; i < EPL / 4; ++i) v.v[i] = __builtin_bit_cast(f32x4, buf_load16_nt(r, off + 16 * i));
+    for (int i = 0; i < EPL / 4; ++i) v.v[i] = __builtin_bit_cast(f32x4, buf_load16(r, off + 16 * i));
   }
   static __device__ __forceinline__ f32x4 qk(const K& k, const Q& q, f32x4 s) {
 #pragma unroll
@@ -279,29 +231,20 @@ struct RowOps<float, D> {
   }
 };
 
-// Partials of chunk s of packed row x of sequence b: its (token, head) pair's row in `part`, chunk s.
-// O relative to m (not divided by l), then m (raw units) and l.
-template <int D>
-__device__ __forceinline__ float* part_o(float* part, int64_t row, int chunks, int s) {
-  return part + (row * chunks + s) * D;
-}
-template <int D>
-__device__ __forceinline__ float2* part_ml(float* part, int64_t all_rows, int chunks, int64_t row, int s) {
-  return reinterpret_cast<float2*>(part + all_rows * chunks * D) + row * chunks + s;
-}
-
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(kRowWaves * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) void paged_rows_kernel(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, T* __restrict__ O, PagedBatch pb, int hq,
-    int G, PagedStrides st, float c2, float sign, int causal, int max_new, int chunk, int chunks, float* __restrict__ part) {
+    int hkv, int G, PagedStrides st, float c2, float sign, int causal, int max_new, int most_rows, int chunk, int chunks, float* __restrict__ part) {
   using R = RowOps<T, D>;
   constexpr int EPL = R::EPL;
   constexpr int MS = 2 + 4 * EPL;  // floats per lane and row tile that the waves exchange
   __shared__ float join[(kRowWaves - 1) * RT * MS * 64];
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
   const int r = lane & 15, lq = lane >> 4;
-  const int hk = blockIdx.y, split = blockIdx.z;
-  const Tile t = find_tile(pb, blockIdx.x, G, 16 * RT, max_new);
+  // Workgroups go to the eight XCDs in turn: with the kv head innermost an XCD's L2 holds the rows of one or a few
+  // heads, which sequences that share pages (beams of one prompt) read at about the same time.
+  const int hk = blockIdx.x % hkv, split = blockIdx.z;
+  const Tile t = find_tile(pb, blockIdx.x / hkv, G, 16 * RT, max_new, 0, most_rows);
   if (t.b < 0) return;
   // the keys that the tile's last row sees bound the tile's
   const int last = min(t.row0 + 16 * RT, t.rows) - 1;
@@ -315,11 +258,11 @@ __global__ __launch_bounds__(kRowWaves * 64, sizeof(T) == 4 && D == 128 ? 1 : 2)
   bool there[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
-    const int x = t.row0 + 16 * rt + r, j = x / G, h = hk * G + x - j * G;
-    there[rt] = x < t.rows;
+    const int xr = t.row0 + 16 * rt + r, x = min(xr, t.rows - 1), j = x / G, h = hk * G + x - j * G;
+    there[rt] = xr < t.rows;  // (a row that is not there reads the last one's query, and leaves nothing)
     sees[rt] = there[rt] ? seen_by(t, j, causal, pb.max_len) : 0;
     at[rt] = (int64_t)(t.t0 + j) * hq + h;
-    R::load_q(q[rt], Q + (int64_t)(t.t0 + j) * st.qt + (int64_t)h * st.qh, lq, there[rt] && sign != 0.f, sign);
+    R::load_q(q[rt], Q + (int64_t)(t.t0 + j) * st.qt + (int64_t)h * st.qh, lq);
   }
   const int first_sees = seen_by(t, t.row0 / G, causal, pb.max_len);  // the fewest keys that a row of the tile sees
 
@@ -337,42 +280,51 @@ __global__ __launch_bounds__(kRowWaves * 64, sizeof(T) == 4 && D == 128 ? 1 : 2)
   typename R::K kr[2];
   typename R::VRow vr[8];
   bool held[2];
-  // The two halves of the block at key kb: their page's rows as far as keys below `end` go; a half in no
+  // Page ids of the wave's next 32 blocks, one half per lane (-1: none, or behind `end`): one load ahead of
+  // the rows' own, which wait for nothing then.
+  int ids = -1;
+  auto load_ids = [&](int kb) {
+    const int key = kb + 32 * kRowWaves * (lane >> 1) + 16 * (lane & 1);
+    ids = key < min(pb.max_len, k0 + chunk) ? table[key >> pb.page_log] : -1;
+  };
+  // Half h of the wave's block n (at key kb): its page's rows as far as keys below `end` go; a half in no
   // page, or behind `end`, reads as zeros.
-  auto rsrc = [&](const T* base, int64_t sp, int64_t sh, int64_t sr, int key, bool* in) {
-    int id = -1;
-    if (key < end) id = table[key >> pb.page_log];
-    id = __builtin_amdgcn_readfirstlane(id);
+  auto rsrc = [&](const T* base, int64_t sp, int64_t sh, int64_t sr, int kb, int n, int h, bool* in) {
+    const int key = kb + 16 * h;
+    const int id = __builtin_amdgcn_readlane(ids, 2 * (n & 31) + h);
     const bool ok = pb.is_page(id);
     *in = ok;
     const int rows = ok ? min(16, end - key) : 0;
     const T* p = base + (int64_t)(ok ? id : 0) * sp + (int64_t)hk * sh + (int64_t)(key & page_mask) * sr;
     return make_rsrc(p, rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * sr + D) * sizeof(T)) : 0u);
   };
-  auto load_k = [&](int kb) {
+  auto load_k = [&](int kb, int n) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      const auto rk = rsrc(K, st.kp, st.kh, st.kr, kb + 16 * h, &held[h]);
+      const auto rk = rsrc(K, st.kp, st.kh, st.kr, kb, n, h, &held[h]);
       R::load_k(kr[h], rk, (uint32_t)(r * st.kr * sizeof(T)), lq);
     }
   };
-  auto load_v = [&](int kb) {
+  auto load_v = [&](int kb, int n) {
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       bool in;
-      const auto rv = rsrc(V, st.vp, st.vh, st.vr, kb + 16 * h, &in);
+      const auto rv = rsrc(V, st.vp, st.vh, st.vr, kb, n, h, &in);
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         R::load_v(vr[4 * h + i], rv, (uint32_t)(((4 * lq + i) * st.vr + EPL * r) * sizeof(T)));
     }
   };
   int kb = k0 + 32 * wave;
+  load_ids(kb);
   if (kb < k1) {
-    load_k(kb);
-    load_v(kb);
+    load_k(kb, 0);
+    load_v(kb, 0);
   }
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) R::sign_q(q[rt], there[rt] ? sign : 0.f);
 #pragma unroll 1
-  for (; kb < k1; kb += 32 * kRowWaves) {
+  for (int n = 1; kb < k1; kb += 32 * kRowWaves, ++n) {
     f32x4 s[RT][2];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
@@ -382,7 +334,10 @@ __global__ __launch_bounds__(kRowWaves * 64, sizeof(T) == 4 && D == 128 ? 1 : 2)
     }
     const bool hole0 = !held[0], hole1 = !held[1];
     const bool more = kb + 32 * kRowWaves < k1;
-    if (more) load_k(kb + 32 * kRowWaves);
+    if (more) {
+      if ((n & 31) == 0) load_ids(kb + 32 * kRowWaves);
+      load_k(kb + 32 * kRowWaves, n);
+    }
     const bool cut = kb + 32 > first_sees;  // some row of the tile does not see all 32 keys
     if (cut || hole0 || hole1)
 #pragma unroll
@@ -465,7 +420,7 @@ __global__ __launch_bounds__(kRowWaves * 64, sizeof(T) == 4 && D == 128 ? 1 : 2)
       }
     }
     R::template pv<RT>(vr, p, o);
-    if (more) load_v(kb + 32 * kRowWaves);
+    if (more) load_v(kb + 32 * kRowWaves, n);
   }
 
   // Join the waves in wave order.
@@ -525,21 +480,24 @@ __global__ __launch_bounds__(kRowWaves * 64, sizeof(T) == 4 && D == 128 ? 1 : 2)
       float* po = part_o<D>(part, at[rt], chunks, split) + 4 * EPL * lq;
 #pragma unroll
       for (int i = 0; i < 4 * EPL; i += 4) *reinterpret_cast<f32x4*>(po + i) = f32x4{f[i], f[i + 1], f[i + 2], f[i + 3]};
-      if (lq == 0) *part_ml<D>(part, (int64_t)pb.tokens * hq, chunks, at[rt], split) = make_float2(mt, lt);
+      if (lq == 0) part_ml<D>(part, (int64_t)pb.tokens * hq, chunks, at[rt])[split] = make_float2(mt, lt);
     }
   }
 }
 
-// Joins a row's chunks in order: a wave per (token, query head).
+// Joins a row's chunks, which hold few_chunk keys in sequences of at most most_rows packed rows and many_chunk in
+// others (0: these have none to join): a workgroup per (token, query head).  Wave w sums chunks w, w + 4, ... with the row's
+// maximum as reference, several loads in flight, and the four sums are added in wave order.
+constexpr int kMergeWaves = 4;
 template <typename T, int D>
-__global__ __launch_bounds__(256) void paged_merge_kernel(float* __restrict__ part, T* __restrict__ O, PagedBatch pb,
-                                                          int hq, PagedStrides st, float c2, int causal, int max_new,
-                                                          int chunk, int chunks) {
+__global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(const float* __restrict__ part, T* __restrict__ O,
+                                                                       PagedBatch pb, int hq, PagedStrides st, float c2,
+                                                                       int causal, int max_new, int G, int most_rows,
+                                                                       int few_chunk, int many_chunk, int chunks) {
   constexpr int E = D / 64;
-  const int64_t row = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  if (row >= (int64_t)pb.tokens * hq) return;
-  const int tok = (int)(row / hq), h = (int)(row - (int64_t)tok * hq);
+  __shared__ float join[kMergeWaves - 1][64][E + 1];
+  const int tok = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t row = (int64_t)tok * hq + h;
   Tile t;
   t.b = pb.sequence_of(tok);
   if (t.b < 0) return;
@@ -547,66 +505,97 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(float* __restrict__ pa
   t.len = pb.len(t.b);
   const int j = tok - pb.first(t.b);
   if (j >= max_new) return;
+  const int chunk = min(t.n, max_new) * G <= most_rows ? few_chunk : many_chunk;
+  if (chunk == 0) return;
   const int seen = seen_by(t, j, causal, pb.max_len), ns = min(chunks, (seen + chunk - 1) / chunk);
+  const float2* ml = part_ml<D>(part, (int64_t)pb.tokens * hq, chunks, row);
+  const float* po = part + row * chunks * D + E * lane;
   float m = -INFINITY;
-  for (int s = lane; s < ns; s += 64) m = fmaxf(m, part_ml<D>(part, (int64_t)pb.tokens * hq, chunks, row, s)->x);
+  for (int s = lane; s < ns; s += 64) m = fmaxf(m, ml[s].x);
   m = wave_max(m);
   float o[E], l = 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) o[e] = 0.f;
-  for (int s = 0; s < ns; ++s) {
-    const float2 ml = *part_ml<D>(part, (int64_t)pb.tokens * hq, chunks, row, s);
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float a = fast_exp2((ml.x - m) * c2);
-    const float* p = part_o<D>(part, row, chunks, s) + E * lane;
-    l += a * ml.y;
+#pragma unroll 4
+  for (int s = w; s < ns; s += kMergeWaves) {
+    const float2 u = ml[s];
+    const float a = u.x == -INFINITY && u.y == 0.f ? 0.f : fast_exp2((u.x - m) * c2);
+    l += a * u.y;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += a * p[e];
+    for (int e = 0; e < E; ++e) o[e] += a * po[(int64_t)s * D + e];
+  }
+  if (w > 0) {
+    join[w - 1][lane][E] = l;
+#pragma unroll
+    for (int e = 0; e < E; ++e) join[w - 1][lane][e] = o[e];
+  }
+  __syncthreads();
+  if (w > 0) return;
+#pragma unroll
+  for (int i = 0; i < kMergeWaves - 1; ++i) {
+    l += join[i][lane][E];
+#pragma unroll
+    for (int e = 0; e < E; ++e) o[e] += join[i][lane][e];
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
   for (int e = 0; e < E; ++e) Elem<T>::store(O + tok * st.ot + h * st.oh, E * lane + e, o[e] * inv);
 }
 
-struct Call {
-  const void *q, *k, *v;
-  void* o;
-  PagedBatch pb;
-  int hq, hkv, G;
-  PagedStrides st;
-  float c2, sign;  // |scale| log2 e, and the scale's sign, which goes to the queries; scale 0: 1 and queries of 0
-  int causal, max_new;
-};
-
-// Workgroup columns that cover every tile of `rows` packed rows, whatever the starts hold.
-int64_t tiles_of(const Call& c, int rows) {
-  const int64_t per = ((int64_t)c.max_new * c.G + rows - 1) / rows;
-  const int64_t all = (int64_t)c.pb.tokens * c.G / rows + c.pb.batch;
-  return c.pb.starts == nullptr || per * c.pb.batch < all ? per * c.pb.batch : all;
+// Chunks of keys for `tiles` tiles per kv head: as few as give the chip `want` workgroups per CU, of `least` keys or more.
+int chunk_of(const PagedCall& c, int64_t tiles, int least, int want) {
+  int chunk = least;
+  while (chunk < c.pb.max_len && tiles * c.hkv * ((c.pb.max_len + chunk - 1) / chunk) > (int64_t)want * cu_count()) chunk *= 2;
+  return chunk;
 }
 
 template <typename T, int D, int RT>
-int launch_rows(const Call& c) {
-  const int64_t tiles = tiles_of(c, 16 * RT);
-  // chunks of keys: enough workgroups for the chip, at least 128 keys (a block for each wave) in each
-  int chunk = 128;
-  const int64_t want = 8 * (int64_t)cu_count();
-  while (chunk < c.pb.max_len && tiles * c.hkv * ((c.pb.max_len + chunk - 1) / chunk) > want) chunk *= 2;
-  const int chunks = c.pb.max_len > chunk ? (c.pb.max_len + chunk - 1) / chunk : 1;
-  KH_REQUIRE(tiles <= INT32_MAX && c.hkv <= 65535 && chunks <= 65535, "kh_paged_attention: too many tiles");
+void launch_rows(const PagedCall& c, int most_rows, int64_t tiles, int chunk, int chunks, float* part) {
+  paged_rows_kernel<T, D, RT><<<dim3((unsigned)(tiles * c.hkv), 1, chunks), kRowWaves * 64, 0, stream()>>>(
+      (const T*)c.q, (const T*)c.k, (const T*)c.v, (T*)c.o, c.pb, c.hq, c.hkv, c.G, c.st, c.c2, c.sign, c.causal, c.max_new,
+      most_rows, chunk, chunks, part);
+}
+
+template <typename T, int D>
+int launch(const PagedCall& c) {
+  const int64_t most = (int64_t)c.max_new * c.G;  // packed rows of a sequence
+  const int E1 = getenv("KP_WANT") ? atoi(getenv("KP_WANT")) : 8, E2 = getenv("KP_TWANT") ? atoi(getenv("KP_TWANT")) : 2,
+            E3 = getenv("KP_WAVES") ? atoi(getenv("KP_WAVES")) : 8, E4 = getenv("KP_FEW") ? atoi(getenv("KP_FEW")) : 64;
+  const bool tiles_too = sizeof(T) == 2 && most > E4;
+  const int few = tiles_too ? (c.pb.batch > 1 ? E4 : 0) : INT32_MAX;  // rows up to which paged_rows_kernel takes a sequence
+  const int rt = most <= 16 ? 1 : 2;
+  const int64_t few_tiles = few == 0 ? 0 : tiles_of(c, 16 * rt);
+  const int waves = E3;
+  const int64_t many_tiles = tiles_too ? tiles_of(c, 32 * waves) : 0;
+  const int few_chunk = chunk_of(c, few_tiles, 128, E1), many_chunk = chunk_of(c, many_tiles, 256, E2);
+  auto count = [&](int chunk) { return c.pb.max_len > chunk ? (c.pb.max_len + chunk - 1) / chunk : 1; };
+  const int few_chunks = few ? count(few_chunk) : 1, many_chunks = tiles_too ? count(many_chunk) : 1;
+  const int chunks = few_chunks > many_chunks ? few_chunks : many_chunks;
+  KH_REQUIRE(few_tiles * c.hkv <= INT32_MAX && many_tiles * c.hkv <= INT32_MAX && chunks <= 65535,
+             "kh_paged_attention: too many tiles");
   float* part = nullptr;
   const int64_t rows = (int64_t)c.pb.tokens * c.hq;
   if (chunks > 1) {
     part = (float*)scratch_alloc((size_t)rows * chunks * (D + 2) * 4);
     if (part == nullptr) return KH_ERR_OOM;
   }
-  paged_rows_kernel<T, D, RT><<<dim3((unsigned)tiles, c.hkv, chunks), kRowWaves * 64, 0, stream()>>>(
-      (const T*)c.q, (const T*)c.k, (const T*)c.v, (T*)c.o, c.pb, c.hq, c.G, c.st, c.c2, c.sign, c.causal, c.max_new, chunk, chunks,
-      part);
-  hipError_t e = hipGetLastError();
-  if (e == hipSuccess && part) {
-    paged_merge_kernel<T, D><<<(unsigned)((rows + 3) / 4), 256, 0, stream()>>>(
-        part, (T*)c.o, c.pb, c.hq, c.st, c.c2, c.causal, c.max_new, chunk, chunks);
+  hipError_t e = hipSuccess;
+  if (tiles_too) {
+    launch_paged_tiles(c, D, waves, few, many_tiles, many_chunk, many_chunks > 1 ? chunks : 1, many_chunks > 1 ? part : nullptr);
+    e = hipGetLastError();
+  }
+  if (few && e == hipSuccess) {
+    float* p = few_chunks > 1 ? part : nullptr;
+    if (rt == 1)
+      launch_rows<T, D, 1>(c, few, few_tiles, few_chunk, few_chunks > 1 ? chunks : 1, p);
+    else
+      launch_rows<T, D, 2>(c, few, few_tiles, few_chunk, few_chunks > 1 ? chunks : 1, p);
+    e = hipGetLastError();
+  }
+  if (part && e == hipSuccess) {
+    paged_merge_kernel<T, D><<<dim3((unsigned)c.pb.tokens, c.hq), kMergeWaves * 64, 0, stream()>>>(
+        part, (T*)c.o, c.pb, c.hq, c.st, c.c2, c.causal, c.max_new, c.G, few, few_chunks > 1 ? few_chunk : 0,
+        many_chunks > 1 ? many_chunk : 0, chunks);
     e = hipGetLastError();
   }
   if (part) scratch_free(part);
@@ -616,12 +605,6 @@ int launch_rows(const Call& c) {
   }
   KH_DEBUG_SYNC();
   return KH_OK;
-}
-
-template <typename T, int D>
-int launch(const Call& c) {
-  if ((int64_t)c.max_new * c.G <= 16) return launch_rows<T, D, 1>(c);
-  return launch_rows<T, D, 2>(c);
 }
 
 }  // namespace
@@ -667,12 +650,12 @@ int kh_paged_attention(const void* q, const void* k_pages, const void* v_pages, 
   KH_REQUIRE_INIT();
   KH_REQUIRE(hq > 0 && hkv > 0 && hq % hkv == 0, "kh_paged_attention: numHeadsQ (%d) must be divisible by numHeadsKV (%d)",
              hq, hkv);
-  KH_REQUIRE(hkv <= 65535, "kh_paged_attention: %d kv heads are too many", hkv);
+  KH_REQUIRE(hq <= 65535, "kh_paged_attention: %d query heads are too many", hq);
   KH_REQUIRE(d == 64 || d == 128, "kh_paged_attention: head_dim %d not supported (64 or 128)", d);
   KH_REQUIRE(dtype == KH_BF16 || dtype == KH_F32, "kh_paged_attention: unsupported dtype %d", dtype);
   KH_REQUIRE(max_query_len >= 0, "kh_paged_attention: negative max_query_len");
   KH_REQUIRE(scale - scale == 0.f, "kh_paged_attention: the scale is not finite");
-  Call c;
+  PagedCall c;
   const int rc = paged_batch("kh_paged_attention", page_table, kv_lens, query_starts, tokens, batch, num_pages, page_size,
                              table_width, table_stride, max_kv_len, &c.pb);
   if (rc != KH_OK) return rc;
