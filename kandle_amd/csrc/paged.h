@@ -134,9 +134,10 @@ inline int64_t tiles_of(const PagedCall& c, int rows) {
 }
 
 // paged_tiles.hip: the call's sequences of more than min_rows packed rows, bfloat16, d 64 or 128, in tiles of
-// 32 `waves` (4 or 8) rows; chunks of `chunk` keys (a multiple of 128), with partials unless there is one.
-void launch_paged_tiles(const PagedCall& c, int d, int waves, int min_rows, int64_t tiles, int chunk, int chunks,
-                        float* part);
+// 32 `waves` (4 or 8) rows; `used` chunks of `chunk` keys (a multiple of 128) each, with partials [rows, chunks]
+// unless part is null.
+void launch_paged_tiles(const PagedCall& c, int d, int waves, int min_rows, int64_t tiles, int chunk, int used,
+                        int chunks, float* part);
 
 inline int log2_of(int64_t v) {
   int n = 0;

@@ -10,7 +10,6 @@
 // Work is split over tiles of packed rows and over chunks of `chunk` keys; where a tile's keys make more
 // than one chunk, each chunk leaves (O, m, l) partials and paged_merge_kernel joins them in chunk order, so
 // a result does not depend on timing.
-#include <cstdlib>
 #include <type_traits>
 
 #include "flash_tiles.h"
@@ -485,31 +484,79 @@ __global__ __launch_bounds__(kRowWaves * 64, sizeof(T) == 4 && D == 128 ? 1 : 2)
   }
 }
 
-// Joins a row's chunks, which hold few_chunk keys in sequences of at most most_rows packed rows and many_chunk in
-// others (0: these have none to join): a workgroup per (token, query head).  Wave w sums chunks w, w + 4, ... with the row's
-// maximum as reference, several loads in flight, and the four sums are added in wave order.
-constexpr int kMergeWaves = 4;
-template <typename T, int D>
-__global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(const float* __restrict__ part, T* __restrict__ O,
-                                                                       PagedBatch pb, int hq, PagedStrides st, float c2,
-                                                                       int causal, int max_new, int G, int most_rows,
-                                                                       int few_chunk, int many_chunk, int chunks) {
-  constexpr int E = D / 64;
-  __shared__ float join[kMergeWaves - 1][64][E + 1];
-  const int tok = blockIdx.x, h = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-  const int64_t row = (int64_t)tok * hq + h;
+// Joins the chunks of a token's query heads, relative to each row's maximum.  Chunks hold few_chunk keys in sequences
+// of at most most_rows packed rows and many_chunk in others (0: these have none to join).
+// Where a row lies and how many chunks it has: of them 0, nothing to do.
+struct MergeArgs {
+  int hq, causal, max_new, G, most_rows, few_chunk, many_chunk, chunks;
+};
+__device__ __forceinline__ int chunks_of(const PagedBatch& pb, const MergeArgs& a, int tok, bool* stored) {
   Tile t;
   t.b = pb.sequence_of(tok);
-  if (t.b < 0) return;
+  *stored = false;
+  if (t.b < 0) return 0;
   t.n = pb.count(t.b);
   t.len = pb.len(t.b);
-  const int j = tok - pb.first(t.b);
-  if (j >= max_new) return;
-  const int chunk = min(t.n, max_new) * G <= most_rows ? few_chunk : many_chunk;
-  if (chunk == 0) return;
-  const int seen = seen_by(t, j, causal, pb.max_len), ns = min(chunks, (seen + chunk - 1) / chunk);
-  const float2* ml = part_ml<D>(part, (int64_t)pb.tokens * hq, chunks, row);
-  const float* po = part + row * chunks * D + E * lane;
+  const int j = tok - pb.first(t.b), chunk = min(t.n, a.max_new) * a.G <= a.most_rows ? a.few_chunk : a.many_chunk;
+  if (j >= a.max_new || chunk == 0) return 0;
+  *stored = true;
+  const int seen = seen_by(t, j, a.causal, pb.max_len);
+  return min(a.chunks, (seen + chunk - 1) / chunk);
+}
+__device__ __forceinline__ float weight_of(float2 ml, float m, float c2) {
+  return ml.x == -INFINITY && ml.y == 0.f ? 0.f : fast_exp2((ml.x - m) * c2);
+}
+
+// Many rows: a workgroup per token, D / 4 lanes per row (query head), so that the token's place is looked up once
+// and several rows' loads are in flight.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void paged_merge_kernel(const float* __restrict__ part, T* __restrict__ O, PagedBatch pb,
+                                                          PagedStrides st, float c2, MergeArgs a) {
+  constexpr int LPR = D / 4, ROWS = 256 / LPR;
+  const int tok = blockIdx.x, lane = threadIdx.x % LPR;
+  bool stored;
+  const int ns = chunks_of(pb, a, tok, &stored);
+  if (!stored) return;
+  const int64_t all = (int64_t)pb.tokens * a.hq;
+  for (int h = threadIdx.x / LPR; h < a.hq; h += ROWS) {
+    const int64_t row = (int64_t)tok * a.hq + h;
+    const float2* ml = part_ml<D>(part, all, a.chunks, row);
+    const float* po = part + row * a.chunks * D + 4 * lane;
+    float m = -INFINITY, l = 0.f;
+    for (int s = 0; s < ns; ++s) m = fmaxf(m, ml[s].x);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int s = 0; s < ns; ++s) {
+      const float2 u = ml[s];
+      const float w = weight_of(u, m, c2);
+      l += w * u.y;
+      o += *reinterpret_cast<const f32x4*>(po + (int64_t)s * D) * w;
+    }
+    const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+    T* to = O + (int64_t)tok * st.ot + (int64_t)h * st.oh + 4 * lane;
+    if constexpr (sizeof(T) == 2)
+      *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16x2(o[0] * inv, o[1] * inv), pack_bf16x2(o[2] * inv, o[3] * inv));
+    else
+      *reinterpret_cast<f32x4*>(to) = o * inv;
+  }
+}
+
+// Few rows: a workgroup per (token, query head); wave w sums chunks w, w + 4, ..., several loads in flight, and the
+// four sums are added in wave order.
+constexpr int kMergeWaves = 4;
+template <typename T, int D>
+__global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_row_kernel(const float* __restrict__ part,
+                                                                           T* __restrict__ O, PagedBatch pb,
+                                                                           PagedStrides st, float c2, MergeArgs a) {
+  constexpr int E = D / 64;
+  __shared__ float join[kMergeWaves - 1][64][E + 1];
+  const int tok = blockIdx.x / a.hq, h = blockIdx.x - tok * a.hq, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const int64_t row = (int64_t)tok * a.hq + h;
+  bool stored;
+  const int ns = chunks_of(pb, a, tok, &stored);
+  if (!stored) return;
+  const float2* ml = part_ml<D>(part, (int64_t)pb.tokens * a.hq, a.chunks, row);
+  const float* po = part + row * a.chunks * D + E * lane;
   float m = -INFINITY;
   for (int s = lane; s < ns; s += 64) m = fmaxf(m, ml[s].x);
   m = wave_max(m);
@@ -519,10 +566,10 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(const flo
 #pragma unroll 4
   for (int s = w; s < ns; s += kMergeWaves) {
     const float2 u = ml[s];
-    const float a = u.x == -INFINITY && u.y == 0.f ? 0.f : fast_exp2((u.x - m) * c2);
-    l += a * u.y;
+    const float f = weight_of(u, m, c2);
+    l += f * u.y;
 #pragma unroll
-    for (int e = 0; e < E; ++e) o[e] += a * po[(int64_t)s * D + e];
+    for (int e = 0; e < E; ++e) o[e] += f * po[(int64_t)s * D + e];
   }
   if (w > 0) {
     join[w - 1][lane][E] = l;
@@ -539,40 +586,56 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_kernel(const flo
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
 #pragma unroll
-  for (int e = 0; e < E; ++e) Elem<T>::store(O + tok * st.ot + h * st.oh, E * lane + e, o[e] * inv);
+  for (int e = 0; e < E; ++e) Elem<T>::store(O + (int64_t)tok * st.ot + (int64_t)h * st.oh, E * lane + e, o[e] * inv);
 }
 
-// Chunks of keys for `tiles` tiles per kv head: as few as give the chip `want` workgroups per CU, of `least` keys or more.
-int chunk_of(const PagedCall& c, int64_t tiles, int least, int want) {
-  int chunk = least;
-  while (chunk < c.pb.max_len && tiles * c.hkv * ((c.pb.max_len + chunk - 1) / chunk) > (int64_t)want * cu_count()) chunk *= 2;
-  return chunk;
+// The length of a chunk of keys: the shortest of least, 2 least, 4 least ... that makes no more than `most` workgroups
+// of `tiles` tiles per kv head, or the whole length.
+int chunk_of(const PagedCall& c, int64_t tiles, int least, int64_t most) {
+  int64_t chunk = least;
+  while (chunk < c.pb.max_len && tiles * c.hkv * ((c.pb.max_len + chunk - 1) / chunk) > most) chunk *= 2;
+  return (int)chunk;
 }
 
 template <typename T, int D, int RT>
-void launch_rows(const PagedCall& c, int most_rows, int64_t tiles, int chunk, int chunks, float* part) {
-  paged_rows_kernel<T, D, RT><<<dim3((unsigned)(tiles * c.hkv), 1, chunks), kRowWaves * 64, 0, stream()>>>(
+void launch_rows(const PagedCall& c, int most_rows, int64_t tiles, int chunk, int used, int chunks, float* part) {
+  paged_rows_kernel<T, D, RT><<<dim3((unsigned)(tiles * c.hkv), 1, used), kRowWaves * 64, 0, stream()>>>(
       (const T*)c.q, (const T*)c.k, (const T*)c.v, (T*)c.o, c.pb, c.hq, c.hkv, c.G, c.st, c.c2, c.sign, c.causal, c.max_new,
       most_rows, chunk, chunks, part);
 }
 
+// Packed rows of a sequence up to which paged_rows_kernel takes it beside paged_tiles.hip: with 160 rows of up to 8000
+// keys (four sequences) it is at 55 us and the tiles at 80, with 96 of 2000 at 19 against 32; with 400 to 512
+// rows the tiles come level (512 of 16384 keys: 59 us against 87).
+constexpr int kFewRows = 256;
+
 template <typename T, int D>
 int launch(const PagedCall& c) {
-  const int64_t most = (int64_t)c.max_new * c.G;  // packed rows of a sequence
-  const int E1 = getenv("KP_WANT") ? atoi(getenv("KP_WANT")) : 8, E2 = getenv("KP_TWANT") ? atoi(getenv("KP_TWANT")) : 2,
-            E3 = getenv("KP_WAVES") ? atoi(getenv("KP_WAVES")) : 8, E4 = getenv("KP_FEW") ? atoi(getenv("KP_FEW")) : 64;
-  const bool tiles_too = sizeof(T) == 2 && most > E4;
-  const int few = tiles_too ? (c.pb.batch > 1 ? E4 : 0) : INT32_MAX;  // rows up to which paged_rows_kernel takes a sequence
+  const int64_t most = (int64_t)c.max_new * c.G, cus = cu_count();
+  // (the tiles take pools of equal strides only)
+  const bool tiles_too =
+      sizeof(T) == 2 && most > kFewRows && c.st.kp == c.st.vp && c.st.kh == c.st.vh && c.st.kr == c.st.vr;
+  // rows up to which paged_rows_kernel takes a sequence; a sequence alone is one or the other's
+  const int few = tiles_too ? (c.pb.batch > 1 ? kFewRows : 0) : INT32_MAX;
   const int rt = most <= 16 ? 1 : 2;
   const int64_t few_tiles = few == 0 ? 0 : tiles_of(c, 16 * rt);
-  const int waves = E3;
-  const int64_t many_tiles = tiles_too ? tiles_of(c, 32 * waves) : 0;
-  const int few_chunk = chunk_of(c, few_tiles, 128, E1), many_chunk = chunk_of(c, many_tiles, 256, E2);
+  // Tiles of 256 rows read K and V half as often as those of 128, of which a CU holds two: better where one
+  // workgroup per CU is all there is and its keys are many (2048 tokens of 16384, 16 / 8 heads: 281 us against
+  // 317), worse with ragged or short ones (four chunks of 512 of 8192: 196 against 179).
+  const int64_t tiles8 = tiles_too ? tiles_of(c, 256) : 0;
+  const int waves = tiles8 * c.hkv <= cus && c.pb.max_len >= 6144 ? 8 : 4;
+  const int64_t many_tiles = !tiles_too ? 0 : (waves == 8 ? tiles8 : tiles_of(c, 128));
+  // Chunks of keys: more workgroups than the chip holds at once, and shorter chunks than 512 keys of a tile, cost
+  // more in partials than they gain (2600 keys of six ragged chunks: 88 us, 98 in twice as many chunks).  The
+  // rows kernel runs two workgroups per CU, one of fp32 at d 128.
+  const int few_chunk = chunk_of(c, few_tiles, 128, 5 * cus * (sizeof(T) == 4 && D == 128 ? 1 : 2) / 4);
+  const int many_chunk = chunk_of(c, many_tiles, 512, waves == 8 ? cus : 2 * cus);
   auto count = [&](int chunk) { return c.pb.max_len > chunk ? (c.pb.max_len + chunk - 1) / chunk : 1; };
   const int few_chunks = few ? count(few_chunk) : 1, many_chunks = tiles_too ? count(many_chunk) : 1;
   const int chunks = few_chunks > many_chunks ? few_chunks : many_chunks;
   KH_REQUIRE(few_tiles * c.hkv <= INT32_MAX && many_tiles * c.hkv <= INT32_MAX && chunks <= 65535,
              "kh_paged_attention: too many tiles");
+  KH_REQUIRE((int64_t)c.pb.tokens * c.hq <= INT32_MAX, "kh_paged_attention: too many rows");
   float* part = nullptr;
   const int64_t rows = (int64_t)c.pb.tokens * c.hq;
   if (chunks > 1) {
@@ -581,21 +644,25 @@ int launch(const PagedCall& c) {
   }
   hipError_t e = hipSuccess;
   if (tiles_too) {
-    launch_paged_tiles(c, D, waves, few, many_tiles, many_chunk, many_chunks > 1 ? chunks : 1, many_chunks > 1 ? part : nullptr);
+    launch_paged_tiles(c, D, waves, few, many_tiles, many_chunk, many_chunks, chunks,
+                       many_chunks > 1 ? part : nullptr);
     e = hipGetLastError();
   }
   if (few && e == hipSuccess) {
     float* p = few_chunks > 1 ? part : nullptr;
     if (rt == 1)
-      launch_rows<T, D, 1>(c, few, few_tiles, few_chunk, few_chunks > 1 ? chunks : 1, p);
+      launch_rows<T, D, 1>(c, few, few_tiles, few_chunk, few_chunks, chunks, p);
     else
-      launch_rows<T, D, 2>(c, few, few_tiles, few_chunk, few_chunks > 1 ? chunks : 1, p);
+      launch_rows<T, D, 2>(c, few, few_tiles, few_chunk, few_chunks, chunks, p);
     e = hipGetLastError();
   }
   if (part && e == hipSuccess) {
-    paged_merge_kernel<T, D><<<dim3((unsigned)c.pb.tokens, c.hq), kMergeWaves * 64, 0, stream()>>>(
-        part, (T*)c.o, c.pb, c.hq, c.st, c.c2, c.causal, c.max_new, c.G, few, few_chunks > 1 ? few_chunk : 0,
-        many_chunks > 1 ? many_chunk : 0, chunks);
+    const MergeArgs a{c.hq,      c.causal, c.max_new, c.G, few, few_chunks > 1 ? few_chunk : 0, many_chunks > 1 ? many_chunk : 0,
+                      chunks};
+    if (c.pb.tokens >= cu_count())
+      paged_merge_kernel<T, D><<<c.pb.tokens, 256, 0, stream()>>>(part, (T*)c.o, c.pb, c.st, c.c2, a);
+    else
+      paged_merge_row_kernel<T, D><<<(unsigned)rows, kMergeWaves * 64, 0, stream()>>>(part, (T*)c.o, c.pb, c.st, c.c2, a);
     e = hipGetLastError();
   }
   if (part) scratch_free(part);

@@ -8,14 +8,17 @@
 //   transposed (ds_read_b64_tr_b16), the softmax relative to a reference that the accumulators start from
 //   (flash_tiles.h) -- the products of the contiguous prefill kernel.
 // What differs is where rows come from: 16 keys lie in one page, the threads of a wave that load together
-// read inside one such block, so a block's page id is a lane's value read as a scalar, and its buffer range
-// ends with the page's rows that the tile sees (others, and blocks in no page, read as zeros).
+// read inside one such block, so a block's place is a lane's value read as scalars (one lane per block, worked
+// out for 1024 keys at once), and its buffer range ends with the page's rows that the tile sees (others, and
+// blocks in no page, read as zeros).  K and V pools have equal strides here.
 #include "flash_tiles.h"
 #include "paged.h"
 
 using namespace kh;
 
 namespace {
+
+typedef uint32_t v4u32 __attribute__((ext_vector_type(4)));
 
 template <int D, int WAVES, int BN>
 struct TileCfg {
@@ -36,6 +39,7 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
     int max_new, int min_rows, int chunk, int chunks, float* __restrict__ part) {
   using C = TileCfg<D, WAVES, BN>;
   __shared__ __attribute__((aligned(16))) uint16_t smem[2 * C::STAGE];
+  __shared__ int odd[2][WAVES];  // whether a wave's V pieces of a tile held infinities or NaN
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
   const int hk = blockIdx.x % hkv, split = blockIdx.z;  // the kv head innermost: an XCD's L2 holds few heads
@@ -52,16 +56,28 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
   const int sees = there ? seen_by(t, j, causal, pb.max_len) : 0;
   const int wave_end = row0 < t.rows ? seen_by(t, (min(row0 + 32, t.rows) - 1) / G, causal, pb.max_len) : 0;
   const int all_see = row0 < t.rows ? seen_by(t, row0 / G, causal, pb.max_len) : 0;
+  const int tile_sees = seen_by(t, t.row0 / G, causal, pb.max_len);  // what every row of the tile sees
 
-  // Page ids of the 64 blocks of 16 keys from key k0 + 1024 w, one per lane, and of the next 64.
+  // A window of 64 blocks of 16 keys, from key k0 + 1024 w, one block per lane: the byte offset of its first row in
+  // the pools (K and V alike: their strides are), the bytes from there that the tile may read, and which
+  // blocks lie in a page at all; and the page id for the next window.
   const int32_t* table = pb.table + t.b * pb.table_stride;
-  const int page_mask = (1 << pb.page_log) - 1;
-  auto ids_of = [&](int w) {
+  auto id_of = [&](int w) {
     const int key = k0 + 1024 * w + 16 * lane;
     return key < k1 ? table[key >> pb.page_log] : -1;
   };
-  int ids = ids_of(0), ids_next = k0 + 1024 < k1 ? ids_of(1) : -1;
-  uint64_t held = __ballot(pb.is_page(ids));  // which of the 64 blocks lie in a page
+  int64_t offs;
+  uint32_t room;
+  uint64_t held;
+  auto window = [&](int w, int id) {
+    const int key = k0 + 1024 * w + 16 * lane, rows = min(16, end - key);
+    const bool ok = pb.is_page(id);
+    offs = ok ? 2 * ((int64_t)id * st.kp + (int64_t)hk * st.kh + (int64_t)(key & ((1 << pb.page_log) - 1)) * st.kr) : 0;
+    room = ok && rows > 0 ? 2u * (uint32_t)((rows - 1) * st.kr + D) : 0u;
+    held = __ballot(ok);
+  };
+  window(0, id_of(0));
+  int id_next = k0 + 1024 < k1 ? id_of(1) : -1;
   bf16x8 qreg[C::NQ];
   {
     const uint16_t* q = Q + (int64_t)(t.t0 + j) * st.qt + (int64_t)h * st.qh + 8 * g;
@@ -73,20 +89,32 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
   constexpr int BSTEP = C::THREADS / C::CPR / 16;
   const int wblk = wave * C::RPW / 16, krow = (tid / C::CPR) & 15, dcol = 8 * (tid % C::CPR);
   uint4 kst[C::NK], vst[C::NK];
-  auto load = [&](const uint16_t* base, int64_t sp, int64_t sh, int64_t sr, int tile, uint4(&to)[C::NK]) {
+  const uint32_t mine = 2u * (uint32_t)(krow * st.kr + dcol);
+  auto load = [&](int tile) {
 #pragma unroll
     for (int i = 0; i < C::NK; ++i) {
-      const int blk = tile * (BN / 16) + wblk + i * BSTEP, key = k0 + 16 * blk;
-      const int id = __builtin_amdgcn_readlane(ids, blk & 63);
-      const bool ok = pb.is_page(id);
-      const int rows = ok ? min(16, end - key) : 0;
-      const uint16_t* p = base + (int64_t)(ok ? id : 0) * sp + (int64_t)hk * sh + (int64_t)(key & page_mask) * sr;
-      const auto rs = make_rsrc(p, rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * sr + D) * 2) : 0u);
-      to[i] = buf_load16(rs, (uint32_t)((krow * sr + dcol) * 2));
+      const int blk = (tile * (BN / 16) + wblk + i * BSTEP) & 63;
+      const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)offs, blk), hi = __builtin_amdgcn_readlane((int)(offs >> 32), blk);
+      const uint32_t bytes = __builtin_amdgcn_readlane((int)room, blk);
+      const int64_t o = (int64_t)(((uint64_t)hi << 32) | lo);
+      kst[i] = buf_load16(make_rsrc((const uint8_t*)K + o, bytes), mine);
+      vst[i] = buf_load16(make_rsrc((const uint8_t*)V + o, bytes), mine);
     }
   };
   auto swap23 = [](int k) { return (k & ~12) | ((k & 4) << 1) | ((k & 8) >> 1); };
-  auto store = [&](uint16_t* stage) {
+  auto store = [&](int tile) {
+    uint16_t* stage = smem + (tile & 1) * C::STAGE;
+    if (k0 + (tile + 1) * BN > tile_sees) {  // rows of the tile see different keys of it: `cut` below
+      bool any = false;
+#pragma unroll
+      for (int i = 0; i < C::NK; ++i) {
+        const v4u32 u = __builtin_bit_cast(v4u32, vst[i]);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) any = any || (u[k] & 0x7f80u) == 0x7f80u || (u[k] & 0x7f800000u) == 0x7f800000u;
+      }
+      const bool found = __any(any);
+      if (lane == 0) odd[tile & 1][wave] = found;
+    }
 #pragma unroll
     for (int i = 0; i < C::NK; ++i) {
       const int key = 16 * (wblk + i * BSTEP) + krow;
@@ -106,10 +134,9 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
   constexpr uint32_t kBits = BN == 128 ? 0xffu : 0xfu;
   uint32_t bits = 0;  // which blocks of the current tile lie in a page
   if (ntiles > 0) {
-    load(K, st.kp, st.kh, st.kr, 0, kst);
-    load(V, st.vp, st.vh, st.vr, 0, vst);
+    load(0);
     bits = (uint32_t)held & kBits;
-    store(smem);
+    store(0);
   }
   {
     const uint32_t flip = sign < 0.f ? 0x80008000u : 0u, keep = there && sign != 0.f ? ~0u : 0u;
@@ -130,12 +157,10 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
     if (more) {
       const int blk = (tile + 1) * (BN / 16);
       if ((blk & 63) == 0) {
-        ids = ids_next;
-        held = __ballot(pb.is_page(ids));
-        ids_next = ids_of(blk / 64 + 1);
+        window(blk / 64, id_next);
+        id_next = id_of(blk / 64 + 1);
       }
-      load(K, st.kp, st.kh, st.kr, tile + 1, kst);
-      load(V, st.vp, st.vh, st.vr, tile + 1, vst);
+      load(tile + 1);
       bits_next = (uint32_t)(held >> (blk & 63)) & kBits;
     }
     const uint16_t* ks = smem + (tile & 1) * C::STAGE;
@@ -185,31 +210,34 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
       sl.l += ps;
       if (cut) {
         // A V row that some of the wave's rows see and others do not may hold infinities or NaN, and 0 times
-        // those is not 0: a chunk that holds any is summed key by key, by the rows that see the key.
-        bool odd = false;
-#pragma unroll 1
-        for (int i = 0; i < C::CPR; ++i) {
-          const uint4 u = *reinterpret_cast<const uint4*>(vs + lane * C::VSTR + 8 * i);
-          const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+        // those is not 0: a chunk of a tile that holds any is summed key by key, by the rows that see the key.
+        int any = 0;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) odd = odd || (w[k] & 0x7f80u) == 0x7f80u || (w[k] & 0x7f800000u) == 0x7f800000u;
-        }
-        if (__any(odd)) {
+        for (int i = 0; i < WAVES; ++i) any |= odd[tile & 1][i];
+        if (__builtin_amdgcn_readfirstlane(any)) {
 #pragma unroll 1
           for (int key = 0; key < 64; ++key) {
-            float p = 0.f;
+            uint32_t word = 0;  // the pair of P values that holds the key's
 #pragma unroll
             for (int k = 0; k < 4; ++k)
 #pragma unroll
-              for (int e = 0; e < 8; ++e)
-                if (k == key >> 4 && e == (key & 7)) p = (float)pk[k][e];
-            p = __shfl(p, r + 32 * ((key >> 3) & 1), 64);
+              for (int e = 0; e < 4; ++e)
+                if (k == key >> 4 && e == ((key >> 1) & 3)) word = __builtin_bit_cast(v4u32, pk[k])[e];
+            word = __shfl(word, r + 32 * ((key >> 3) & 1), 64);
+            const float p = (key & 1) ? hi_bf16(word) : lo_bf16(word);
             if (kt + key < sees && ((pages >> (key >> 4)) & 1u)) {
+              const uint16_t* v = vs + key * C::VSTR + 4 * g;
 #pragma unroll
               for (int dt = 0; dt < C::ND; ++dt)
 #pragma unroll
-                for (int i = 0; i < 16; ++i)
-                  oacc[dt][i] += p * bf16_bits_to_f32(vs[key * C::VSTR + 32 * dt + 8 * (i >> 2) + 4 * g + (i & 3)]);
+                for (int a = 0; a < 4; ++a) {
+                  const uint2 u = *reinterpret_cast<const uint2*>(v + 32 * dt + 8 * a);
+                  oacc[dt][4 * a] += p * lo_bf16(u.x);
+                  oacc[dt][4 * a + 1] += p * hi_bf16(u.x);
+                  oacc[dt][4 * a + 2] += p * lo_bf16(u.y);
+                  oacc[dt][4 * a + 3] += p * hi_bf16(u.y);
+                  __builtin_amdgcn_sched_barrier(0);  // (few registers here: the loop's staged rows are live)
+                }
             }
           }
           continue;
@@ -239,7 +267,7 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
       }
       mfma_block_end();
     }
-    if (more) store(smem + ((tile + 1) & 1) * C::STAGE);
+    if (more) store(tile + 1);
     bits = bits_next;
     __syncthreads();
   }
@@ -273,8 +301,8 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
 }
 
 template <int D, int WAVES, int BN, int MINB>
-void launch_tiles(const PagedCall& c, int min_rows, int64_t tiles, int chunk, int chunks, float* part) {
-  paged_tiles_kernel<D, WAVES, BN, MINB><<<dim3((unsigned)(tiles * c.hkv), 1, chunks), WAVES * 64, 0, stream()>>>(
+void launch_tiles(const PagedCall& c, int min_rows, int64_t tiles, int chunk, int used, int chunks, float* part) {
+  paged_tiles_kernel<D, WAVES, BN, MINB><<<dim3((unsigned)(tiles * c.hkv), 1, used), WAVES * 64, 0, stream()>>>(
       (const uint16_t*)c.q, (const uint16_t*)c.k, (const uint16_t*)c.v, (uint16_t*)c.o, c.pb, c.hq, c.hkv, c.G, c.st, c.c2,
       c.sign, c.causal, c.max_new, min_rows, chunk, chunks, part);
 }
@@ -283,18 +311,18 @@ void launch_tiles(const PagedCall& c, int min_rows, int64_t tiles, int chunk, in
 
 namespace kh {
 
-void launch_paged_tiles(const PagedCall& c, int d, int waves, int min_rows, int64_t tiles, int chunk, int chunks,
-                        float* part) {
+void launch_paged_tiles(const PagedCall& c, int d, int waves, int min_rows, int64_t tiles, int chunk, int used,
+                        int chunks, float* part) {
   if (d == 128) {
     if (waves == 8)
-      launch_tiles<128, 8, 128, 1>(c, min_rows, tiles, chunk, chunks, part);
+      launch_tiles<128, 8, 128, 1>(c, min_rows, tiles, chunk, used, chunks, part);
     else
-      launch_tiles<128, 4, 64, 2>(c, min_rows, tiles, chunk, chunks, part);
+      launch_tiles<128, 4, 64, 2>(c, min_rows, tiles, chunk, used, chunks, part);
   } else {
     if (waves == 8)
-      launch_tiles<64, 8, 128, 1>(c, min_rows, tiles, chunk, chunks, part);
+      launch_tiles<64, 8, 128, 1>(c, min_rows, tiles, chunk, used, chunks, part);
     else
-      launch_tiles<64, 4, 64, 2>(c, min_rows, tiles, chunk, chunks, part);
+      launch_tiles<64, 4, 64, 2>(c, min_rows, tiles, chunk, used, chunks, part);
   }
 }
 

@@ -29,19 +29,16 @@ def paged_attention(q, k_pages, v_pages, table, kv_lens, starts=None, scale=None
         rows = rows[(ids >= 0) & (ids < pages)]
         ids = table[b, rows // page]
         k, v = kp[ids, :, rows % page], vp[ids, :, rows % page]
-        for j in range(n):
-            see = rows <= length - n + j if causal else np.ones(len(rows), bool)
-            for h in range(hq):
-                hk = h // (hq // hkv)
-                if not see.any():
-                    o[t0 + j, h] = 0
-                    continue
-                s = scale * (k[see, hk] @ q[t0 + j, h])
-                p = np.exp(s - s.max())
-                p /= p.sum()
-                o[t0 + j, h] = p @ v[see, hk]
-                a[t0 + j, h] = p @ np.abs(v[see, hk])
-                smax[t0 + j, h] = abs(scale) * (np.abs(k[see, hk]) @ np.abs(q[t0 + j, h])).max()
+        see = rows[None] <= (length - n + np.arange(n))[:, None] if causal else np.ones((n, len(rows)), bool)
+        none = ~see.any(1)
+        for h in range(hq):
+            hk, mine = h // (hq // hkv), q[t0:t0 + n, h]
+            p = np.where(see, scale * (mine @ k[:, hk].T), -np.inf)
+            p = np.exp(p - np.where(none, 0, p.max(1, initial=-np.inf))[:, None])
+            p /= np.where(none, 1, p.sum(1))[:, None]
+            o[t0:t0 + n, h] = p @ v[:, hk]
+            a[t0:t0 + n, h] = p @ np.abs(v[:, hk])
+            smax[t0:t0 + n, h] = abs(scale) * np.where(see, np.abs(mine) @ np.abs(k[:, hk]).T, 0).max(1, initial=0)
     return o, a, smax
 
 

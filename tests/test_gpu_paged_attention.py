@@ -75,6 +75,8 @@ def test_one_token_per_sequence(hip, dtype, hq, hkv, d, page):
     (34, 2, 64, 16, [77, 200], [5, 40]),
     (8, 8, 64, 16, [600, 1, 40], [300, 1, 0]),
     (4, 1, 128, 256, [1100], [513]),
+    (4, 2, 128, 16, [7000], [300]),              # 256-row tiles
+    (8, 2, 64, 32, [6500, 6300], [70, 100]),
     (2, 2, 128, 16, [2300, 9], [7, 9]),
 ])
 def test_ragged_chunks(hip, dtype, hq, hkv, d, page, lens, news):
@@ -139,7 +141,7 @@ def test_rows_outside_the_sequences_stay_and_limits_hold(hip, dtype, news):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("news,hq", [([1, 1], 4), ([16, 5], 4), ([40, 300], 4), ([40, 300], 24)])
+@pytest.mark.parametrize("news,hq", [([1, 1], 4), ([16, 5], 4), ([40, 300], 4), ([40, 300], 24), ([200, 2], 8)])
 @pytest.mark.parametrize("poison", [np.nan, np.inf, -np.inf])
 def test_values_in_masked_places_do_not_matter(hip, dtype, news, hq, poison):
     """Rows behind the cached ones, pages of nobody, and later tokens' rows may hold anything."""
@@ -189,7 +191,7 @@ def test_a_nan_query_stays_in_its_row(hip, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("news", [[1, 1], [50, 7]])
+@pytest.mark.parametrize("news", [[1, 1], [50, 7], [200, 7]])
 def test_large_scores(hip, dtype, news):
     """Scores of hundreds, growing along the sequence: the running maximum has to follow."""
     c = Cache(43, dtype, [500, 260], 2, 64, 16)
@@ -226,11 +228,21 @@ def test_strided_operands(hip, dtype, news):
     compare(c, wh[:, 4:10], out.numpy(), st)
 
 
+@pytest.mark.parametrize("news", [[150, 2, 1], [300, 700, 1]])
+def test_pools_with_the_heads_inside_the_rows(hip, news):
+    """Equal strides of keys and values other than the usual: [pages, page size, heads, d] seen with heads first."""
+    c = Cache(48, "bfloat16", [1300, 720, 31], 3, 128, 32)
+    turn = lambda x: F.permute(dev(np.ascontiguousarray(x.transpose(0, 2, 1, 3)), "bfloat16"), (0, 2, 1, 3))  # noqa: E731
+    c.k, c.v = turn(c.kh), turn(c.vh)
+    check(c, 50, news, 6)
+    check(c, 52, news, 6, causal=False)
+
+
 def test_offsets_beyond_32_bits(hip):
     """A pool of 2^31 elements and more: pages at its far end."""
     page, d, pages = 16, 128, (1 << 20) + 5000
     k, v = F.zeros((pages, 1, page, d), "bfloat16"), F.zeros((pages, 1, page, d), "bfloat16")
-    for lens, news in (([70, 500], [1, 1]), ([70, 500], [40, 300])):
+    for lens, news in (([70, 500], [1, 1]), ([70, 500], [40, 30]), ([70, 500], [40, 300])):
         c = Cache(51, "bfloat16", lens, 1, d, page, spare=0)
         far = pages - c.kh.shape[0]
         for big, small in ((k, c.k), (v, c.v)):
