@@ -32,7 +32,7 @@ from __future__ import annotations
 import time
 from collections import OrderedDict
 from dataclasses import dataclass, field
-from typing import Dict, List, Optional
+from typing import Dict, List, Optional, Sequence
 
 import numpy as np
 
@@ -45,6 +45,7 @@ from ..graphs import HipGraph
 from ..kernels import TensorIterator, interleave_gate_up
 from ..tensor import HipTensorHandle, Tensor
 from .kv_cache import StaticKVCache
+from .paged_cache import PagedKVCache
 from .rope import RotaryEmbedding
 
 
@@ -236,6 +237,7 @@ class Qwen3ForCausalLM:
         # qk-norm, RoPE and the K/V cache write in its epilogue (linear_qk_norm_rope, head_dim 128;
         # the same values); False always runs the projection and rms_norm_rope as two launches.
         self.fused_qkv_rope = cfg.head_dim == 128
+        self._rows: Dict[int, Tensor] = {}   # row count -> its arange on the device
 
     # -- decoder body shared by the prefill and the device-resident decode step -------------------
     @classmethod
@@ -259,9 +261,13 @@ class Qwen3ForCausalLM:
         model.load_result = result
         return model
 
-    def _decoder(self, x: Tensor, S: int, positions: Tensor, attend, decode_block: bool = False) -> Tensor:
+    def _decoder(self, x: Tensor, S: int, positions: Tensor, attend, decode_block: bool = False, heads=None,
+                 pick: Optional[Tensor] = None) -> Tensor:
         """Runs every decoder layer over the fp32 residual rows x [S, hidden] in place and returns
-        the fp32 logits of the last position [1, vocab].  positions: int32 [S] device tensor
+        the fp32 logits of the last position [1, vocab].  heads(layer, weights, qkv) replaces the
+        attention from the QKV projection (which it disposes) to the heads [S, nq], for a cache that
+        `attend` does not know; pick (int32 [n], on the device) names other rows whose logits [n, vocab]
+        are wanted.  positions: int32 [S] device tensor
         (RoPE angles and KV-cache rows); attend(layer, q_heads, out_view) writes attention for
         q_heads [1, Hq, S, D] into out_view [1, Hq, S, D].  A single row (decode) runs each norm
         and the SwiGLU product inside the projection that consumes it (linear_fused); with
@@ -282,7 +288,7 @@ class Qwen3ForCausalLM:
         # The fused QKV projection sums each output over all of K, as kh_gemm does when it takes
         # its MFMA tiles (more than 8 rows) without splitting K: only then are the values the same.
         nqkv = (cfg.num_attention_heads + 2 * cfg.num_key_value_heads) * cfg.head_dim
-        fuse_qkv = (self.fused_qkv_rope and not one and S > 8
+        fuse_qkv = (self.fused_qkv_rope and heads is None and not one and S > 8
                     and gemm_split_count(S, nqkv, Hd, act) == 1)
         # the RoPE angles of these positions, once for every layer's fused projection
         rope_tab = self.ops.find("rope_table")(positions.handle, self.rope.inv_freq.handle) if fuse_qkv else None
@@ -297,7 +303,7 @@ class Qwen3ForCausalLM:
                 qkv.dispose()
             elif one:
                 qkv = F.linear_fused("rms_norm", x, L["w_qkv"], L["in_norm"], eps, act_dtype=act)  # [1, nq + 2 nkv]
-                attn_t = self._attention_heads(li, L, qkv, S, positions, attend)
+                attn_t = self._attention_heads(li, L, qkv, S, positions, attend) if heads is None else heads(li, L, qkv)
                 F.linear_fused("none", attn_t, L["w_o"], residual=x, act_dtype=act)     # x += o W_o^T
                 attn_t.dispose()
             elif fuse_qkv:
@@ -308,7 +314,7 @@ class Qwen3ForCausalLM:
             else:
                 qkv = F.linear(h, L["w_qkv"])                                          # [S, nq + 2 nkv]
                 h.dispose()
-                attn_t = self._attention_heads(li, L, qkv, S, positions, attend)
+                attn_t = self._attention_heads(li, L, qkv, S, positions, attend) if heads is None else heads(li, L, qkv)
                 h = F.linear_add_rms_norm(attn_t, L["w_o"], x, L["post_norm_a"], eps)   # x += o W_o^T
                 attn_t.dispose()
             if one:
@@ -322,7 +328,8 @@ class Qwen3ForCausalLM:
                 if li + 1 < n_layers:
                     h = F.linear_add_rms_norm(a, L["w_down"], x, self.layers[li + 1]["in_norm_a"], eps)
                 else:
-                    h = F.linear_add_rms_norm(a, L["w_down"], x, self.final_norm_a, eps, rows=(S - 1, S))
+                    h = F.linear_add_rms_norm(a, L["w_down"], x, self.final_norm_a, eps,
+                                              rows=(S - 1, S) if pick is None else None)
                 a.dispose()
         if rope_tab is not None:
             rope_tab.dispose()
@@ -332,7 +339,11 @@ class Qwen3ForCausalLM:
                                     act_dtype=act)
             last.dispose()
         else:
-            logits = F.linear(h, self.lm_head, out_dtype="float32")                    # [1, vocab] fp32
+            if pick is not None:
+                picked = F.index_select(h, 0, pick)
+                h.dispose()
+                h = picked
+            logits = F.linear(h, self.lm_head, out_dtype="float32")                    # [1 or n, vocab] fp32
             h.dispose()
         return logits
 
@@ -414,6 +425,179 @@ class Qwen3ForCausalLM:
         for t in (ids, positions):
             t.dispose()
         return logits
+
+    # -- many sequences over a paged cache ----------------------------------------------------------
+    def new_paged_cache(self, max_sequences: int, num_pages: int, max_seq_len: Optional[int] = None,
+                        page_size: int = 16) -> PagedKVCache:
+        """A paged cache for this model's layers, in its activation dtype."""
+        c = self.cfg
+        return PagedKVCache(c.num_hidden_layers, c.num_key_value_heads, c.head_dim, num_pages, max_sequences,
+                            self.max_seq_len if max_seq_len is None else max_seq_len, page_size, self.act)
+
+    def _paged_dev(self, ids: Tensor, positions: Tensor, starts: Optional[Tensor], pick: Optional[Tensor],
+                   cache: PagedKVCache, max_new: int, max_len: int) -> Tensor:
+        """Logits [n, vocab] of the rows `pick` (None: every row) of the packed new tokens ids [T] at `positions`, whose
+        rows the cache has been made room for; starts None: one token per sequence."""
+        cfg = self.cfg
+        T, Hq, Hkv, D = ids.shape[0], cfg.num_attention_heads, cfg.num_key_value_heads, cfg.head_dim
+        nq, nkv = Hq * D, Hkv * D
+        x = F.embedding(ids, self.embed, out_dtype="float32")
+
+        def heads(li, L, qkv):
+            parts = [_split_heads(qkv, o, T, n, D) for o, n in ((0, Hq), (nq, Hkv), (nq + nkv, Hkv))]
+            # q and k normalised and rotated into [T, heads, D] rows; k and v from there into their pages
+            rows = [HipTensorHandle.create_new((T, n, D), self.act) for n in (Hq, Hkv)]
+            first = [HipTensorHandle.create_view(r.storage, (1, n, T, D), self.act, (T * n * D, D, n * D, 1), 0)
+                     for r, n in zip(rows, (Hq, Hkv))]
+            self.ops.find("rms_norm_rope")(parts[0].handle, parts[1].handle, {
+                "q_weight": L["q_norm_a"].handle, "k_weight": L["k_norm_a"].handle, "inv_freq": self.rope.inv_freq.handle,
+                "positions": positions.handle, "eps": cfg.rms_norm_eps, "q_out": first[0], "k_out": first[1]})
+            q, k = (Tensor(handle=r) for r in rows)
+            v = Tensor(handle=HipTensorHandle.create_view(qkv.handle.storage, (T, Hkv, D), self.act, (nq + 2 * nkv, D, 1),
+                                                          parts[2].offset))
+            kp, vp = cache.layer(li)
+            F.paged_kv_write(k, v, kp, vp, cache.page_table, cache.kv_lens, starts)
+            o = F.paged_attention(q, kp, vp, cache.page_table, cache.kv_lens, starts, scale=self.scale,
+                                  max_query_len=max_new, max_kv_len=max_len)
+            out = F.view(o, (T, nq))
+            for t in (*parts, *first, q, k, v, o, qkv):
+                t.dispose()
+            return out
+
+        logits = self._decoder(x, T, positions, None, heads=heads, pick=pick if pick is not None else self._every_row(T))
+        x.dispose()
+        return logits
+
+    def _every_row(self, n: int) -> Optional[Tensor]:
+        rows = self._rows.get(n)
+        if rows is None:
+            rows = self._rows[n] = Tensor(np.arange(n, dtype=np.int32), dtype="int32")
+        return rows
+
+    def forward_paged(self, input_ids: Sequence[int], counts: Sequence[int], cache: PagedKVCache) -> Tensor:
+        """One serving step: counts[s] new tokens (0: none) for each of the cache's sequences, packed in input_ids in
+        that order -- chunks of prompts, single tokens, or both together.  Returns the fp32 logits [n, vocab]
+        of the last new token of each sequence that has any.  Raises, with the cache unchanged, if the new
+        rows do not fit."""
+        ids_h, n = np.asarray(input_ids, np.int32).reshape(-1), cache._check_counts(counts)
+        if len(ids_h) != n.sum() or not len(ids_h):
+            raise ValueError(f"forward_paged: {len(ids_h)} tokens for counts that sum to {n.sum()}")
+        before = cache.lens.copy()
+        cache.reserve(n)
+        starts_h = np.concatenate([[0], np.cumsum(n)])
+        pos_h = np.concatenate([np.arange(b, b + c) for b, c in zip(before, n)])
+        ids, positions, starts, pick = (Tensor(np.ascontiguousarray(a, np.int32), dtype="int32") for a in
+                                        (ids_h, pos_h, starts_h, starts_h[1:][n > 0] - 1))
+        logits = self._paged_dev(ids, positions, starts, pick, cache, int(n.max()), int(cache.lens[n > 0].max()))
+        for t in (ids, positions, starts, pick):
+            t.dispose()
+        return logits
+
+    def generate_beams(self, prompts, num_beams: int, max_new_tokens: int, eos_token_id: Optional[int] = None,
+                       length_penalty: float = 1.0, page_size: int = 16, num_pages: Optional[int] = None,
+                       use_graph: bool = True):
+        """Beam search: for each prompt its num_beams best continuations of up to max_new_tokens tokens, best first,
+        as lists of (tokens, score).  At every step the num_beams continuations with the highest sum of
+        log-probabilities go on; one that has reached eos_token_id (which it ends with) stays as it is, and a
+        group stops when all of its have.  The returned order and score are sum / length ** length_penalty.
+
+        The prompts go through the model once, as one ragged batch; beams share their prompt's pages and
+        whatever else they have in common.  Selection, the beams' page bookkeeping and the forward of a step run on
+        the device; with use_graph they are captured (two steps: the page tables change places) and replayed, and
+        the host reads a step's tokens and parents back to follow them."""
+        prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        G, B, N = len(prompts), int(num_beams), int(max_new_tokens)
+        if not G or not all(len(p) for p in prompts) or B < 1 or N < 1:
+            raise ValueError("generate_beams: prompts of one token or more, one beam or more, one new token or more expected")
+        if B > min(64, self.cfg.vocab_size):
+            raise ValueError(f"generate_beams: {B} beams, at most {min(64, self.cfg.vocab_size)}")
+        if eos_token_id is not None and not 0 <= eos_token_id < self.cfg.vocab_size:
+            raise ValueError(f"generate_beams: eos_token_id {eos_token_id} outside [0, {self.cfg.vocab_size})")
+        S, longest = G * B, max(len(p) for p in prompts)
+        if longest + N > self.max_seq_len:
+            raise ValueError(f"Cache overflow: trying to write to position {longest}-{longest + N}, but maxSeqLen is {self.max_seq_len}")
+        if num_pages is None:   # the prompts' full pages once, and what each beam may add to them
+            num_pages = sum(len(p) // page_size for p in prompts) + S * (-(-(N + page_size) // page_size) + 1)
+        cache = self.new_paged_cache(S, num_pages, longest + N, page_size)
+        i32 = lambda a: Tensor(np.ascontiguousarray(a, np.int32), dtype="int32")  # noqa: E731
+        base = i32(np.repeat(np.arange(G)[:, None] * B, B, 1))
+        ones, scores, finished = i32(np.ones(S)), F.zeros((G, B)), F.zeros((G, B), "int32")
+        tokens, parents, rows = (F.zeros(s, "int32") for s in ((G, B), (G, B), (S,)))
+        own = [cache, base, ones, scores, finished, tokens, parents, rows]
+        flags = finished if eos_token_id is not None else None
+        graphs, kept, history = [], [], []
+
+        def step():
+            """One step on device state: the beams' tokens through the model, the next choice, and the rows after it."""
+            cache.enqueue_reserve(ones)
+            pos = F.sub(cache.kv_lens, ones)
+            lg = self._paged_dev(F.view(tokens, (S,)), pos, None, None, cache, 1, longest + N)
+            pos.dispose()
+            o = F.beam_select(F.view(lg, (G, B, self.cfg.vocab_size)), scores, B, flags, eos_token_id)
+            for dst, src in ((scores, o[0]), (tokens, o[1]), (parents, o[2]), (finished, o[3])):
+                if src is not None:
+                    F.copy_(dst, src)
+                    src.dispose()
+            r = F.add(parents, base)
+            F.copy_(rows, F.view(r, (S,)))
+            r.dispose()
+            cache.enqueue_fork(rows)
+            return lg
+
+        try:
+            counts = np.zeros(S, np.int64)
+            counts[::B] = [len(p) for p in prompts]
+            lg = self.forward_paged(np.concatenate(prompts), counts, cache)
+            # the first choice: each group's best continuations of its one prompt, whose rows all its beams take over
+            zero = F.zeros((G, 1))
+            o = F.beam_select(F.view(lg, (G, 1, self.cfg.vocab_size)), zero, B)
+            for dst, src in ((scores, o[0]), (tokens, o[1])):
+                F.copy_(dst, src)
+            if flags is not None:
+                finished.handle.storage.upload((tokens.numpy() == eos_token_id).astype(np.int32))
+            F.copy_(rows, F.view(base, (S,)))
+            cache.enqueue_fork(rows)
+            for t in (lg, zero, *o[:3]):
+                t.dispose()
+            for i in range(N):
+                t, p, f = tokens.numpy(), parents.numpy(), finished.numpy()
+                history.append((t, p))
+                if i + 1 == N or (flags is not None and f.all()):
+                    break
+                if not use_graph or i < 2:
+                    step().dispose()
+                else:
+                    if len(graphs) < 2:   # the odd steps' tables and the even ones': capture records, replay runs
+                        g = HipGraph()
+                        with g.capture():
+                            kept.append(step())
+                        graphs.append(g)
+                        cache.state, cache._other = cache._other, cache.state
+                    graphs[i % 2].replay()
+                    cache.state, cache._other = cache._other, cache.state
+                cache.check_info()
+            total = scores.numpy()
+        finally:
+            for t in kept:
+                t.dispose()
+            for g in graphs:
+                g.dispose()
+            for t in own:
+                t.dispose()
+        out = []
+        for gi in range(G):
+            beams = []
+            for b in range(B):
+                toks, at = [], b
+                for t, p in reversed(history):
+                    toks.append(int(t[gi, at]))
+                    at = int(p[gi, at])
+                toks.reverse()
+                if eos_token_id is not None and eos_token_id in toks:
+                    toks = toks[:toks.index(eos_token_id) + 1]
+                beams.append((toks, float(total[gi, b]) / len(toks) ** length_penalty))
+            out.append(sorted(beams, key=lambda x: -x[1]))
+        return out
 
     def _prefill(self, prompt_ids: np.ndarray, use_graph: bool):
         """(logits, owned) of the prompt at position 0.  With use_graph, the first prompt of a given
@@ -632,6 +816,8 @@ class Qwen3ForCausalLM:
         for key in list(self._prefill_graphs):
             self._dispose_prefill_graph(key)
         self.cache.dispose()
+        for t in self._rows.values():
+            t.dispose()
         heads = [self.lm_head] if self.lm_head is not self.embed else []
         extra = [self.final_norm_a] if self.final_norm_a is not self.final_norm else []
         owned = {}
