@@ -30,10 +30,52 @@ __device__ __forceinline__ uint64_t order_bits(double x) {
 __device__ __forceinline__ double order_value(uint64_t u) {
   return __longlong_as_double((long long)((u >> 63) ? (u & 0x7fffffffffffffffull) : ~u));
 }
-__device__ __forceinline__ float no_nan(float x) { return x != x ? -INFINITY : x; }
+__device__ __forceinline__ float no_nan(float x) { return fmaxf(x, -INFINITY); }
 
-// A candidate: the larger `hi` first, then the lower `at`.  hi 0: none.  Logits hold their order bits in the
-// upper half of hi; the merge holds those of a float64 score.
+// A logit's key inside its beam: the larger logit first, then the lower id.
+__device__ __forceinline__ uint64_t order_key(float x, int id) {
+  return ((uint64_t)order_bits(x) << 32) | (uint64_t)(0xffffffffu - (uint32_t)id);
+}
+__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) {
+    const uint64_t u = __shfl_xor(v, o, 64);
+    v = u > v ? u : v;
+  }
+  return v;
+}
+__device__ __forceinline__ float wave_max_dpp(float v) {
+  v = fmaxf(v, dpp_f<0xB1>(v));
+  v = fmaxf(v, dpp_f<0x4E>(v));
+  v = fmaxf(v, dpp_f<0x141>(v));
+  v = fmaxf(v, dpp_f<0x140>(v));
+  const int b = __builtin_bit_cast(int, v);
+  return fmaxf(fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 0)), __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 16))),
+               fmaxf(__builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 32)), __builtin_bit_cast(float, __builtin_amdgcn_readlane(b, 48))));
+}
+// Place of this lane among those whose bit is set in `who`.
+__device__ __forceinline__ int place_in(uint64_t who) {
+  return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+}
+
+// The selections below start from the k-th largest of the 64 lanes' maxima: k candidates are at least as large, so
+// nothing below it is among the k largest, and a handful above it are left, which are ranked by counting.
+// It is found bit by bit with ballots, and may be left lower as soon as exactly k lanes are above.  Where more
+// than kRoom candidates are left (many equal values), k rounds of a wave-wide maximum do the same.
+constexpr int kRoom = 128;
+__device__ __forceinline__ uint32_t kth_lane(uint32_t top, int k) {
+  uint32_t floor = 0;
+  for (int b = 31; b >= 0; --b) {
+    const uint32_t t = floor | (1u << b);
+    const int n = __popcll(__ballot(top >= t));
+    if (n >= k) floor = t;
+    if (n == k) break;
+  }
+  return floor;
+}
+
+// A candidate of the merge: the larger `hi` (order bits of a float64 score) first, then the lower `at` (beam *
+// vocab + token).  hi 0: none.
 struct Cand {
   uint64_t hi;
   int64_t at;
@@ -42,32 +84,20 @@ __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.
 
 // The k best of a wave's candidates, N per lane in registers, in order to out[0 .. k) (LDS; none behind the
 // last); `room` is the wave's own LDS for kRoom candidates.
-//
-// The k-th largest of the lanes' maxima (of hi's upper word) is at most the k-th largest candidate, so
-// nothing below it is wanted; a handful above it are left, which are ranked by counting.  It is found bit
-// by bit with ballots.  Where more than kRoom are left (many equal values), k rounds of a wave-wide
-// maximum do the same.
-constexpr int kRoom = 128;
 template <int N>
 __device__ __forceinline__ void wave_best(Cand (&c)[N], int k, Cand* room, Cand* out) {
   const int lane = threadIdx.x & 63;
   uint32_t top = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) top = max(top, (uint32_t)(c[i].hi >> 32));
-  uint32_t floor = 0;
-  for (int b = 31; b >= 0; --b) {
-    const uint32_t t = floor | (1u << b);
-    const int n = __popcll(__ballot(top >= t));
-    if (n >= k) floor = t;
-    if (n == k) break;
-  }
+  const uint32_t floor = kth_lane(top, k);
   int count = 0;
 #pragma unroll
   for (int i = 0; i < N; ++i) {
     const bool keep = c[i].hi != 0 && (uint32_t)(c[i].hi >> 32) >= floor;
     const uint64_t who = __ballot(keep);
     if (who != 0) {
-      const int at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+      const int at = count + place_in(who);
       if (keep && at < kRoom) room[at] = c[i];
       count += __popcll(who);
     }
@@ -112,19 +142,19 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
                                                                    const int32_t* __restrict__ finished, int k, int runs,
                                                                    float2* __restrict__ sums, uint64_t* __restrict__ keys) {
   constexpr int E = 16 / sizeof(T);
-  __shared__ Cand room[kRunWaves][kRoom];
-  __shared__ Cand best[kRunWaves * kMaxK];
+  __shared__ uint64_t room[kRunWaves][kRoom];
+  __shared__ uint64_t best[kRunWaves * kMaxK];
   __shared__ float2 part[kRunWaves];
   const int row = blockIdx.y, run = blockIdx.x, lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   if (finished && finished[row] != 0) return;
   const T* x = logits + (int64_t)(row / beams) * sg + (int64_t)(row % beams) * sb;
   const int shift = (int)(((uintptr_t)x & 15) / sizeof(T));
-  const int64_t start = (int64_t)run * kRun + w * (kRun / kRunWaves) + lane * E - shift;
+  const int start = run * kRun + w * (kRun / kRunWaves) + lane * E - shift;  // id of the lane's first value
   float v[kPer];
 #pragma unroll
   for (int j = 0; j < kPer / E; ++j) {
-    const int64_t id = start + j * 64 * E;
+    const int id = start + j * 64 * E;
     if (id >= 0 && id + E <= vocab) {
       const uint4 u = *reinterpret_cast<const uint4*>(x + id);
       if constexpr (E == 4) {
@@ -143,26 +173,62 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
       for (int e = 0; e < E; ++e) v[E * j + e] = id + e >= 0 && id + e < vocab ? Elem<T>::load(x, id + e) : -INFINITY;
     }
   }
-  float m = -INFINITY;
+  // id of value i; values behind the row's end are -inf like some inside it, and told apart by it
+  auto id_of = [&](int i) { return start + (i / E) * 64 * E + i % E; };
+  float mine = -INFINITY;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     v[i] = no_nan(v[i]);
-    m = fmaxf(m, v[i]);
+    mine = fmaxf(mine, v[i]);
   }
-  m = wave_max(m);
+  const float m = wave_max_dpp(mine);
   float s = 0.f;
-  if (m > -INFINITY)
+  if (m > -INFINITY) {
 #pragma unroll
     for (int i = 0; i < kPer; ++i) s += fast_exp2((v[i] - m) * kLog2e);
-  s = wave_sum(s);
-  Cand c[kPer];
+    s = wave_sum(s);
+  }
+  if (lane == 0) part[w] = make_float2(m, s);
+  // the wave's k best as order keys, in order
+  uint64_t* out = best + w * k;
+  const float floor = order_value(kth_lane(order_bits(mine), k));
+  int count = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
-    const int64_t id = start + (int64_t)(i / E) * 64 * E + i % E;
-    c[i] = Cand{id >= 0 && id < vocab ? (uint64_t)order_bits(v[i]) << 32 : 0, id};
+    bool keep = v[i] >= floor;
+    if (__ballot(keep) != 0) {
+      const int id = id_of(i);
+      keep = keep && id >= 0 && id < vocab;
+      const uint64_t who = __ballot(keep);
+      const int at = count + place_in(who);
+      if (keep && at < kRoom) room[w][at] = order_key(v[i], id);
+      count += __popcll(who);
+    }
   }
-  wave_best<kPer>(c, k, room[w], best + w * k);
-  if (lane == 0) part[w] = make_float2(m, s);
+  for (int j = lane; j < k; j += 64) out[j] = 0;
+  __builtin_amdgcn_wave_barrier();
+  if (count <= kRoom) {
+    for (int j = lane; j < count; j += 64) {
+      const uint64_t key = room[w][j];
+      int rank = 0;
+      for (int i = 0; i < count; ++i) rank += room[w][i] > key;
+      if (rank < k) out[rank] = key;
+    }
+  } else {
+    uint64_t last = ~0ull;  // the one chosen last
+    for (int j = 0; j < k; ++j) {
+      uint64_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int id = id_of(i);
+        const uint64_t key = id >= 0 && id < vocab ? order_key(v[i], id) : 0;
+        if (key < last && key > top) top = key;
+      }
+      last = wave_max_u64(top);
+      if (lane == 0) out[j] = last;
+      if (last == 0) break;
+    }
+  }
   __syncthreads();
   const int64_t o = (int64_t)row * runs + run;
   if (threadIdx.x == 0) {
@@ -174,15 +240,12 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
       if (part[i].x > -INFINITY) ss += part[i].y * fast_exp2((part[i].x - mm) * kLog2e);
     sums[o] = make_float2(mm, ss);
   }
-  // the waves' best joined: each is ranked among all
+  // the waves' best joined: each is ranked among all (keys differ, but for the zeros behind the last)
   for (int j = threadIdx.x; j < kRunWaves * k; j += kRunWaves * 64) {
-    const Cand mine = best[j];
+    const uint64_t key = best[j];
     int rank = 0;
-    for (int i = 0; i < kRunWaves * k; ++i) {
-      const Cand u = best[i];
-      rank += before(u, mine) || (u.hi == 0 && mine.hi == 0 && i < j);
-    }
-    if (rank < k) keys[o * k + rank] = mine.hi == 0 ? 0 : mine.hi | (uint32_t)mine.at;
+    for (int i = 0; i < kRunWaves * k; ++i) rank += best[i] > key || (best[i] == key && i < j);
+    if (rank < k) keys[o * k + rank] = key;
   }
 }
 
@@ -241,7 +304,8 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
         } else {
           const uint64_t key = keys[(int64_t)(g * beams + b) * per + n];
           if (key != 0)
-            c[i] = Cand{order_bits((double)order_value((uint32_t)(key >> 32)) + base[b]), (int64_t)b * vocab + (uint32_t)key};
+            c[i] = Cand{order_bits((double)order_value((uint32_t)(key >> 32)) + base[b]),
+                        (int64_t)b * vocab + (int64_t)(0xffffffffu - (uint32_t)key)};
         }
       }
     }
@@ -249,12 +313,15 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
     wave_best<kSlots + 1>(c, k, room[w], mine);
   }
   __syncthreads();
-  for (int j = threadIdx.x; j < kMergeWaves * k; j += kMergeWaves * 64) {
+  // the waves' best ranked among all, sixteen lanes to each
+  for (int j = threadIdx.x / 16; j < kMergeWaves * k; j += kMergeWaves * 4) {
     const Cand u = best[j];
-    if (u.hi == 0) continue;
     int rank = 0;
-    for (int i = 0; i < kMergeWaves * k; ++i) rank += before(best[i], u);
-    if (rank >= k) continue;
+    if (u.hi != 0)
+      for (int i = threadIdx.x & 15; i < kMergeWaves * k; i += 16) rank += before(best[i], u);
+#pragma unroll
+    for (int off = 8; off > 0; off >>= 1) rank += __shfl_xor(rank, off, 16);
+    if (u.hi == 0 || rank >= k || (threadIdx.x & 15) != 0) continue;
     const int b = (int)(u.at / vocab), t = (int)(u.at - (int64_t)b * vocab), o = g * k + rank;
     out_scores[o] = (float)order_value(u.hi);
     out_tokens[o] = t;
@@ -274,7 +341,7 @@ int kh_beam_select(const void* logits, const int64_t* strides, const float* scor
   KH_REQUIRE(dtype == KH_BF16 || dtype == KH_F32, "kh_beam_select: unsupported dtype %d", dtype);
   KH_REQUIRE(groups >= 0 && groups <= 65535 && beams >= 1 && beams <= kMaxBeams && groups * beams <= 65535,
              "kh_beam_select: %lld groups of %lld beams (1 to %d beams, at most 65535 rows)", (long long)groups, (long long)beams, kMaxBeams);
-  KH_REQUIRE(vocab >= 1 && vocab < INT32_MAX - kRun, "kh_beam_select: bad vocabulary size %lld", (long long)vocab);
+  KH_REQUIRE(vocab >= 1 && vocab < INT32_MAX - 2 * kRun, "kh_beam_select: bad vocabulary size %lld", (long long)vocab);
   KH_REQUIRE(k >= 1 && k <= kMaxK, "kh_beam_select: k %d outside 1..%d", k, kMaxK);
   KH_REQUIRE((finished != nullptr) == (out_finished != nullptr), "kh_beam_select: finished flags go in and come out together");
   // a group whose beams have all finished has that many continuations
