@@ -87,8 +87,8 @@ def decode_attention(q: Tensor, k_cache: Tensor, v_cache: Tensor, seq_lens: Tens
 # paged KV cache and beam search
 # ---------------------------------------------------------------------------------------------
 def _limit(name: str, what: str, v) -> Optional[int]:
-    if v is None:
-        return None
+    if v is None or type(v) is int and v >= 0:
+        return v
     if isinstance(v, bool) or int(v) != v or v < 0:
         raise ValueError(f"{name}: {what} must be a non-negative integer, got {v!r}")
     return int(v)

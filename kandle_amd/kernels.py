@@ -1112,6 +1112,20 @@ def philox4x32_10(seed: int, counters, out) -> None:
 # paged KV cache
 # ---------------------------------------------------------------------------------------------
 _NO_LIMIT = (1 << 63) - 1
+_plans: dict = {}  # (kernel, operands' dtypes, shapes and strides) -> the checked call's extents and strides
+
+
+def _plan(make, *handles):
+    """make(*handles), a kernel's checks of its operands and what follows for its call, once per geometry: a step
+    repeats the same shapes for every layer, and checking costs more host time than the launch."""
+    key = (make, *[None if h is None else (h.dtype, h.shape, h.strides) for h in handles])
+    plan = _plans.get(key)
+    if plan is None:
+        plan = make(*handles)
+        if len(_plans) >= 1024:
+            _plans.clear()
+        _plans[key] = plan
+    return plan
 
 
 def _int32(name: str, what: str, h, shape) -> None:
@@ -1121,21 +1135,19 @@ def _int32(name: str, what: str, h, shape) -> None:
                          f"{h.dtype} {list(h.shape)}")
 
 
-def _page_table(name: str, table) -> None:
+def _page_table(name: str, table) -> int:
+    """The table's row stride."""
     if table.dtype != INT32 or len(table.shape) != 2 or (table.shape[1] > 1 and table.strides[1] != 1):
         raise ValueError(f"{name}: page_table must be an int32 tensor [sequences, pages] with contiguous rows, got "
                          f"{table.dtype} {list(table.shape)}")
     if table.shape[0] > 1 and table.strides[0] < table.shape[1]:
         raise ValueError(f"{name}: page_table's rows must not overlap")
-
-
-def _row_stride(table) -> int:
     return table.strides[0] if table.shape[0] > 1 else table.shape[1]
 
 
 def _token_rows(name: str, what: str, h, heads: int, d: int) -> list:
     """(token, head) strides of a [tokens, heads, d] tensor with contiguous rows."""
-    if len(h.shape) != 3 or h.shape[1] != heads or h.shape[2] != d or not (_last_dim_contiguous(h)):
+    if len(h.shape) != 3 or h.shape[1] != heads or h.shape[2] != d or not _last_dim_contiguous(h):
         raise ValueError(f"{name}: {what} must be [tokens, {heads}, {d}] with a contiguous last dim, got {list(h.shape)}")
     return [h.strides[0], h.strides[1]]
 
@@ -1148,23 +1160,19 @@ def _pools(name: str, k_pages, v_pages) -> list:
     return list(k_pages.strides[:3]) + list(v_pages.strides[:3])
 
 
-def _sequences(name: str, table, kv_lens, query_starts, tokens: int) -> int:
-    """The batch size; the arrays' shapes checked."""
-    _page_table(name, table)
+def _sequences(name: str, table, kv_lens, query_starts, tokens: int) -> list:
+    """Batch size, table width and row stride; the arrays' shapes checked."""
+    stride = _page_table(name, table)
     B = table.shape[0]
     _int32(name, "kv_lens", kv_lens, (B,))
     if query_starts is not None:
         _int32(name, "query_starts", query_starts, (B + 1,))
     elif tokens != B:
         raise ValueError(f"{name}: without query_starts every sequence has one new token ({tokens} tokens, {B} sequences)")
-    return B
+    return [B, table.shape[1], stride]
 
 
-def paged_attention(query, key_pages, value_pages, page_table, kv_lens, query_starts, output, scale: float,
-                    is_causal: bool, max_query_len=None, max_kv_len=None) -> None:
-    """Attention of a ragged batch's new tokens over a paged cache (kh_paged_attention): query / output
-    [tokens, Hq, D], pools [pages, Hkv, page size, D], page_table int32 [B, W], kv_lens int32 [B],
-    query_starts int32 [B + 1] or None (one token each).  Rows behind the last sequence stay as they were."""
+def _paged_attention_plan(query, key_pages, value_pages, output, table, kv_lens, query_starts):
     dt = query.dtype
     if dt not in (FLOAT32, BFLOAT16) or key_pages.dtype != dt or value_pages.dtype != dt or output.dtype != dt:
         raise TypeError(f"paged_attention: query, pages and output must share float32 or bfloat16, got {dt}, "
@@ -1180,19 +1188,26 @@ def paged_attention(query, key_pages, value_pages, page_table, kv_lens, query_st
         raise ValueError(f"paged_attention: output has {output.shape[0]} tokens, query {tokens}")
     if hkv == 0 or hq % hkv != 0:
         raise ValueError(f"paged_attention: numHeadsQ ({hq}) must be divisible by numHeadsKV ({hkv})")
+    B, width, stride = _sequences("paged_attention", table, kv_lens, query_starts, tokens)
+    return tokens, B, hq, hkv, d, n_pages, page, width, stride, _lib.i64_array(qs + pools + os_), query.kh_dtype
+
+
+def paged_attention(query, key_pages, value_pages, page_table, kv_lens, query_starts, output, scale: float,
+                    is_causal: bool, max_query_len=None, max_kv_len=None) -> None:
+    """Attention of a ragged batch's new tokens over a paged cache (kh_paged_attention): query / output
+    [tokens, Hq, D], pools [pages, Hkv, page size, D], page_table int32 [B, W], kv_lens int32 [B],
+    query_starts int32 [B + 1] or None (one token each).  Rows behind the last sequence stay as they were."""
+    (tokens, B, hq, hkv, d, n_pages, page, width, stride, strides, dtype) = _plan(
+        _paged_attention_plan, query, key_pages, value_pages, output, page_table, kv_lens, query_starts)
     if not math.isfinite(scale):
         raise ValueError(f"paged_attention: scale {scale} is not finite")
-    B = _sequences("paged_attention", page_table, kv_lens, query_starts, tokens)
     _lib.call("kh_paged_attention", query.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), output.data_ptr(),
               page_table.data_ptr(), kv_lens.data_ptr(), None if query_starts is None else query_starts.data_ptr(), tokens, B,
-              hq, hkv, d, n_pages, page, page_table.shape[1], _row_stride(page_table),
-              _lib.i64_array(qs + pools + os_), scale, 1 if is_causal else 0,
-              _NO_LIMIT if max_query_len is None else max_query_len, _NO_LIMIT if max_kv_len is None else max_kv_len,
-              query.kh_dtype)
+              hq, hkv, d, n_pages, page, width, stride, strides, scale, 1 if is_causal else 0,
+              _NO_LIMIT if max_query_len is None else max_query_len, _NO_LIMIT if max_kv_len is None else max_kv_len, dtype)
 
 
-def paged_kv_write(key, value, key_pages, value_pages, page_table, kv_lens, query_starts) -> None:
-    """The new tokens' rows key / value [tokens, Hkv, D] into their pages (kh_paged_kv_write)."""
+def _paged_kv_write_plan(key, value, key_pages, value_pages, table, kv_lens, query_starts):
     dt = key.dtype
     if dt not in (FLOAT32, BFLOAT16) or value.dtype != dt or key_pages.dtype != dt or value_pages.dtype != dt:
         raise TypeError(f"paged_kv_write: rows and pages must share float32 or bfloat16, got {dt}, {value.dtype}, "
@@ -1203,10 +1218,15 @@ def paged_kv_write(key, value, key_pages, value_pages, page_table, kv_lens, quer
     tokens = key.shape[0]
     if value.shape[0] != tokens:
         raise ValueError(f"paged_kv_write: key has {tokens} tokens, value {value.shape[0]}")
-    B = _sequences("paged_kv_write", page_table, kv_lens, query_starts, tokens)
+    B, width, stride = _sequences("paged_kv_write", table, kv_lens, query_starts, tokens)
+    return tokens, B, hkv, d, n_pages, page, width, stride, _lib.i64_array(st + pools), key.kh_dtype
+
+
+def paged_kv_write(key, value, key_pages, value_pages, page_table, kv_lens, query_starts) -> None:
+    """The new tokens' rows key / value [tokens, Hkv, D] into their pages (kh_paged_kv_write)."""
+    plan = _plan(_paged_kv_write_plan, key, value, key_pages, value_pages, page_table, kv_lens, query_starts)
     _lib.call("kh_paged_kv_write", key.data_ptr(), value.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
-              page_table.data_ptr(), kv_lens.data_ptr(), None if query_starts is None else query_starts.data_ptr(), tokens, B,
-              hkv, d, n_pages, page, page_table.shape[1], _row_stride(page_table), _lib.i64_array(st + pools), key.kh_dtype)
+              page_table.data_ptr(), kv_lens.data_ptr(), None if query_starts is None else query_starts.data_ptr(), *plan)
 
 
 def _page_refs(name: str, page_refs) -> int:
@@ -1215,36 +1235,45 @@ def _page_refs(name: str, page_refs) -> int:
     return page_refs.shape[0]
 
 
-def pages_fork(page_table, kv_lens, page_refs, parents, new_table, new_lens, new_refs) -> None:
-    """Rows of a page table follow their parents (kh_pages_fork)."""
-    _page_table("pages_fork", page_table)
-    rows, width = page_table.shape
+def _pages_fork_plan(table, kv_lens, page_refs, parents, new_table, new_lens, new_refs):
+    stride = _page_table("pages_fork", table)
+    rows, width = table.shape
     n = _page_refs("pages_fork", page_refs)
     for what, h in (("kv_lens", kv_lens), ("parents", parents), ("the new kv_lens", new_lens)):
         _int32("pages_fork", what, h, (rows,))
     _int32("pages_fork", "the new page_table", new_table, (rows, width))
     _int32("pages_fork", "the new page_refs", new_refs, (n,))
-    _lib.call("kh_pages_fork", page_table.data_ptr(), _row_stride(page_table), kv_lens.data_ptr(), page_refs.data_ptr(),
-              parents.data_ptr(), rows, width, n, new_table.data_ptr(), new_lens.data_ptr(), new_refs.data_ptr())
+    return stride, rows, width, n
 
 
-def pages_reserve(page_table, kv_lens, page_refs, counts, page_size: int, moves, info) -> None:
-    """Rows of a page table grow, in place (kh_pages_reserve)."""
-    _page_table("pages_reserve", page_table)
-    rows, width = page_table.shape
+def pages_fork(page_table, kv_lens, page_refs, parents, new_table, new_lens, new_refs) -> None:
+    """Rows of a page table follow their parents (kh_pages_fork)."""
+    stride, rows, width, n = _plan(_pages_fork_plan, page_table, kv_lens, page_refs, parents, new_table, new_lens, new_refs)
+    _lib.call("kh_pages_fork", page_table.data_ptr(), stride, kv_lens.data_ptr(), page_refs.data_ptr(), parents.data_ptr(),
+              rows, width, n, new_table.data_ptr(), new_lens.data_ptr(), new_refs.data_ptr())
+
+
+def _pages_reserve_plan(table, kv_lens, page_refs, counts, moves, info):
+    stride = _page_table("pages_reserve", table)
+    rows, width = table.shape
     n = _page_refs("pages_reserve", page_refs)
     for what, h in (("kv_lens", kv_lens), ("counts", counts)):
         _int32("pages_reserve", what, h, (rows,))
     _int32("pages_reserve", "moves", moves, (rows, 2))
     _int32("pages_reserve", "info", info, (3,))
-    _lib.call("kh_pages_reserve", page_table.data_ptr(), _row_stride(page_table), kv_lens.data_ptr(), page_refs.data_ptr(),
-              counts.data_ptr(), rows, width, n, page_size, moves.data_ptr(), info.data_ptr())
+    return stride, rows, width, n
 
 
-def pages_compact(page_table, page_refs, new_table, new_refs, moves, info) -> None:
-    """Where the live pages go when they move to the front of the pool (kh_pages_compact)."""
-    _page_table("pages_compact", page_table)
-    rows, width = page_table.shape
+def pages_reserve(page_table, kv_lens, page_refs, counts, page_size: int, moves, info) -> None:
+    """Rows of a page table grow, in place (kh_pages_reserve)."""
+    stride, rows, width, n = _plan(_pages_reserve_plan, page_table, kv_lens, page_refs, counts, moves, info)
+    _lib.call("kh_pages_reserve", page_table.data_ptr(), stride, kv_lens.data_ptr(), page_refs.data_ptr(), counts.data_ptr(),
+              rows, width, n, page_size, moves.data_ptr(), info.data_ptr())
+
+
+def _pages_compact_plan(table, page_refs, new_table, new_refs, moves, info):
+    stride = _page_table("pages_compact", table)
+    rows, width = table.shape
     n = _page_refs("pages_compact", page_refs)
     _int32("pages_compact", "the new page_table", new_table, (rows, width))
     _int32("pages_compact", "the new page_refs", new_refs, (n,))
@@ -1252,13 +1281,17 @@ def pages_compact(page_table, page_refs, new_table, new_refs, moves, info) -> No
         raise ValueError(f"pages_compact: moves must be int32 [at least {n // 2}, 2], got {list(moves.shape)}")
     _int32("pages_compact", "moves", moves, (moves.shape[0], 2))
     _int32("pages_compact", "info", info, (2,))
-    _lib.call("kh_pages_compact", page_table.data_ptr(), _row_stride(page_table), page_refs.data_ptr(), rows, width, n,
-              new_table.data_ptr(), new_refs.data_ptr(), moves.data_ptr(), moves.shape[0], info.data_ptr())
+    return stride, rows, width, n
 
 
-def pages_copy(pages, moves, info) -> None:
-    """Page moves[i, 0] to page moves[i, 1] for i < info[0], in every pool of pages [..., num_pages, Hkv,
-    page size, D] (kh_pages_copy)."""
+def pages_compact(page_table, page_refs, new_table, new_refs, moves, info) -> None:
+    """Where the live pages go when they move to the front of the pool (kh_pages_compact)."""
+    stride, rows, width, n = _plan(_pages_compact_plan, page_table, page_refs, new_table, new_refs, moves, info)
+    _lib.call("kh_pages_compact", page_table.data_ptr(), stride, page_refs.data_ptr(), rows, width, n, new_table.data_ptr(),
+              new_refs.data_ptr(), moves.data_ptr(), moves.shape[0], info.data_ptr())
+
+
+def _pages_copy_plan(pages, moves, info):
     if len(pages.shape) < 4 or not pages.is_contiguous():
         raise ValueError(f"pages_copy: pages must be contiguous [..., pages, kv heads, page size, head dim], got {list(pages.shape)}")
     if len(moves.shape) != 2:
@@ -1267,13 +1300,17 @@ def pages_copy(pages, moves, info) -> None:
     if info.dtype != INT32 or len(info.shape) != 1 or info.shape[0] < 1 or not info.is_contiguous():
         raise ValueError(f"pages_copy: info must be an int32 tensor whose first value is the number of moves, got {info.dtype} {list(info.shape)}")
     sh = pages.shape
-    _lib.call("kh_pages_copy", pages.data_ptr(), math.prod(sh[:-4]), sh[-4], sh[-3] * sh[-2] * sh[-1] * pages.itemsize,
-              moves.data_ptr(), moves.shape[0], info.data_ptr())
+    return math.prod(sh[:-4]), sh[-4], sh[-3] * sh[-2] * sh[-1] * pages.itemsize
 
 
-def beam_select(logits, scores, finished, k: int, eos_token_id, out_scores, out_tokens, out_parents, out_finished) -> None:
-    """The k best continuations of each group of beams (kh_beam_select): logits [groups, beams, vocab],
-    scores float32 [groups, beams], finished int32 [groups, beams] or None; outputs [groups, k]."""
+def pages_copy(pages, moves, info) -> None:
+    """Page moves[i, 0] to page moves[i, 1] for i < info[0], in every pool of pages [..., num_pages, Hkv,
+    page size, D] (kh_pages_copy)."""
+    planes, n, page_bytes = _plan(_pages_copy_plan, pages, moves, info)
+    _lib.call("kh_pages_copy", pages.data_ptr(), planes, n, page_bytes, moves.data_ptr(), moves.shape[0], info.data_ptr())
+
+
+def _beam_select_plan(logits, scores, finished, out_scores, out_tokens, out_parents, out_finished):
     if logits.dtype not in (FLOAT32, BFLOAT16):
         raise TypeError(f"beam_select: logits dtype {logits.dtype} not supported (float32 or bfloat16)")
     if len(logits.shape) != 3 or not _last_dim_contiguous(logits):
@@ -1281,21 +1318,31 @@ def beam_select(logits, scores, finished, k: int, eos_token_id, out_scores, out_
     groups, beams, vocab = logits.shape
     if scores.dtype != FLOAT32 or scores.shape != (groups, beams) or not scores.is_contiguous():
         raise ValueError(f"beam_select: scores must be contiguous float32 [{groups}, {beams}], got {scores.dtype} {list(scores.shape)}")
+    if out_scores.dtype != FLOAT32 or len(out_scores.shape) != 2 or out_scores.shape[0] != groups or not out_scores.is_contiguous():
+        raise ValueError(f"beam_select: the new scores must be contiguous float32 [{groups}, k], got {list(out_scores.shape)}")
+    k = out_scores.shape[1]
     if (finished is None) != (out_finished is None):
         raise ValueError("beam_select: finished flags go in and come out together")
     if finished is not None:
         _int32("beam_select", "finished", finished, (groups, beams))
         _int32("beam_select", "the new finished", out_finished, (groups, k))
-        if eos_token_id is None:
-            raise ValueError("beam_select: finished beams need an eos_token_id")
-    if out_scores.dtype != FLOAT32 or out_scores.shape != (groups, k) or not out_scores.is_contiguous():
-        raise ValueError(f"beam_select: the new scores must be contiguous float32 [{groups}, {k}]")
     _int32("beam_select", "tokens", out_tokens, (groups, k))
     _int32("beam_select", "parents", out_parents, (groups, k))
-    _lib.call("kh_beam_select", logits.data_ptr(), _lib.i64_array(logits.strides[:2]), scores.data_ptr(),
-              None if finished is None else finished.data_ptr(), groups, beams, vocab, k,
-              -1 if eos_token_id is None else eos_token_id, out_scores.data_ptr(), out_tokens.data_ptr(), out_parents.data_ptr(),
-              None if out_finished is None else out_finished.data_ptr(), logits.kh_dtype)
+    return _lib.i64_array(logits.strides[:2]), groups, beams, vocab, k, logits.kh_dtype
+
+
+def beam_select(logits, scores, finished, k: int, eos_token_id, out_scores, out_tokens, out_parents, out_finished) -> None:
+    """The k best continuations of each group of beams (kh_beam_select): logits [groups, beams, vocab],
+    scores float32 [groups, beams], finished int32 [groups, beams] or None; outputs [groups, k]."""
+    strides, groups, beams, vocab, k_out, dtype = _plan(_beam_select_plan, logits, scores, finished, out_scores, out_tokens,
+                                                        out_parents, out_finished)
+    if k != k_out:
+        raise ValueError(f"beam_select: results of {k_out} continuations for k = {k}")
+    if finished is not None and eos_token_id is None:
+        raise ValueError("beam_select: finished beams need an eos_token_id")
+    _lib.call("kh_beam_select", logits.data_ptr(), strides, scores.data_ptr(), None if finished is None else finished.data_ptr(),
+              groups, beams, vocab, k, -1 if eos_token_id is None else eos_token_id, out_scores.data_ptr(),
+              out_tokens.data_ptr(), out_parents.data_ptr(), None if out_finished is None else out_finished.data_ptr(), dtype)
 
 
 KERNELS = {
