@@ -133,11 +133,17 @@ inline int64_t tiles_of(const PagedCall& c, int rows) {
   return c.pb.starts == nullptr || per * c.pb.batch < all ? per * c.pb.batch : all;
 }
 
-// paged_tiles.hip: the call's sequences of more than min_rows packed rows, bfloat16, d 64 or 128, in tiles of
-// 32 `waves` (4 or 8) rows; `used` chunks of `chunk` keys (a multiple of 128) each, with partials [rows, chunks]
-// unless part is null.
-void launch_paged_tiles(const PagedCall& c, int d, int waves, int min_rows, int64_t tiles, int chunk, int used,
-                        int chunks, float* part);
+// How a launch form covers its sequences: workgroups for `columns` (tiles x kv heads) by `used` chunks of `chunk` keys.
+struct PagedPart {
+  int columns, chunk, used;
+};
+
+// paged_tiles.hip, bfloat16, d 64 or 128: every sequence in tiles of 32 `waves` (4 or 8) packed rows; or sequences of more
+// than few_rows of them in tiles of 128, the others in tiles of 32.  Chunks are multiples of 128 keys, with
+// partials in part [rows, chunks] where a form uses more than one.
+void launch_paged_tiles(const PagedCall& c, int d, int waves, const PagedPart& many, int chunks, float* part);
+void launch_paged_mixed(const PagedCall& c, int d, int few_rows, const PagedPart& many, const PagedPart& few, int chunks,
+                        float* part);
 
 inline int log2_of(int64_t v) {
   int n = 0;

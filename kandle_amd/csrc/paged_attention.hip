@@ -10,478 +10,20 @@
 // Work is split over tiles of packed rows and over chunks of `chunk` keys; where a tile's keys make more
 // than one chunk, each chunk leaves (O, m, l) partials and paged_merge_kernel joins them in chunk order, so
 // a result does not depend on timing.
-#include <type_traits>
-
-#include "flash_tiles.h"
-#include "paged.h"
+#include "paged_rows.h"
 
 using namespace kh;
 
 namespace {
 
-// ---- few rows: K and V straight from the pages into MFMA operands --------------------------------
-//
-// A workgroup of four waves takes one tile of 16 RT packed rows of one kv head and one chunk of keys; wave
-// w takes the chunk's 32-key blocks w, w + 4, ...  A 32-key block is two 16-key halves, each inside one
-// page (pages are multiples of 16 rows), so its page id and base address are wave-uniform.
-//
-//   S^T (16 keys x 16 rows) = K Q^T with v_mfma_f32_16x16x32_bf16 (or _16x16x4_f32): lane (r, q), r =
-//     lane % 16, q = lane / 16, loads K row r of the half, columns 32 c + 8 q .. + 7 (fp32: 16 c + 4 q .. + 3)
-//     and gets the scores of packed row r with keys 4 q + i.
-//   O^T += V^T P^T: the k slots of the product may hold the keys in any order that P and V share, so lane
-//     (r, q) keeps the P values it has (keys 4 q + i of both halves) and loads the V rows of those keys, D/16
-//     consecutive columns EPL r ..: 16 lanes read a whole row.  Tile dt of O^T has the columns EPL r + dt.
-// Nothing passes through LDS until the waves' (m, l, O) are joined at the end.
-//
-// Softmax relative to a reference maximum m (raw q . k units) that the accumulators start from, raised
-// only when a lane's sum of P exceeds kSumMax, as in the contiguous prefill kernel: O / l does not depend on
-// it, and P <= kSumMax holds whatever the scores are.
-constexpr int kRowWaves = 4;
-
-template <typename T, int D>
-struct RowOps;
-
-// bfloat16
-template <int D>
-struct RowOps<uint16_t, D> {
-  static constexpr int NK = D / 32, EPL = D / 16;
-  struct K {
-    uint4 v[NK];
-  };
-  using VRow = std::conditional_t<EPL == 8, uint4, uint2>;
-  struct Q {
-    bf16x8 v[NK];
-  };
-  // A query row, and the row times sign (0: zeros whatever it holds).
-  static __device__ __forceinline__ void load_q(Q& q, const uint16_t* row, int lq) {
-#pragma unroll
-    for (int c = 0; c < NK; ++c)
-      q.v[c] = __builtin_bit_cast(bf16x8, *reinterpret_cast<const uint4*>(row + 32 * c + 8 * lq));
-  }
-  static __device__ __forceinline__ void sign_q(Q& q, float sign) {
-    const uint32_t flip = sign < 0.f ? 0x80008000u : 0u, keep = sign != 0.f ? ~0u : 0u;
-#pragma unroll
-    for (int c = 0; c < NK; ++c) {
-      uint4 u = __builtin_bit_cast(uint4, q.v[c]);
-      u.x = (u.x ^ flip) & keep;
-      u.y = (u.y ^ flip) & keep;
-      u.z = (u.z ^ flip) & keep;
-      u.w = (u.w ^ flip) & keep;
-      q.v[c] = __builtin_bit_cast(bf16x8, u);
-    }
-  }
-  static __device__ __forceinline__ void load_k(K& k, __amdgpu_buffer_rsrc_t r, uint32_t off, int lq) {
-#pragma unroll
-    for (int c = 0; c < NK; ++c) k.v[c] = buf_load16(r, off + 64 * c + 16 * lq);
-  }
-  static __device__ __forceinline__ void load_v(VRow& v, __amdgpu_buffer_rsrc_t r, uint32_t off) {
-    if constexpr (EPL == 8)
-      v = buf_load16(r, off);
-    else
-      v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
-  }
-  static __device__ __forceinline__ f32x4 qk(const K& k, const Q& q, f32x4 s) {
-#pragma unroll
-    for (int c = 0; c < NK; ++c)
-      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k.v[c]), q.v[c], s, 0, 0, 0);
-    return s;
-  }
-  static __device__ __forceinline__ uint32_t word(const VRow& v, int w) {
-    if constexpr (EPL == 8)
-      return w == 0 ? v.x : (w == 1 ? v.y : (w == 2 ? v.z : v.w));
-    else
-      return w == 0 ? v.x : v.y;
-  }
-  // P of one row tile as the products take it, and the lane's sum of those values.
-  struct P {
-    bf16x8 v;
-  };
-  static __device__ __forceinline__ float exponentiate(const f32x4 (&s)[2], float c2, P& p) {
-    float sum = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const __bf16 b = (__bf16)fast_exp2(s[h][i] * c2);
-        p.v[4 * h + i] = b;
-        sum += (float)b;
-      }
-    return sum;
-  }
-  template <int RT>
-  static __device__ __forceinline__ void pv(const VRow (&v)[8], const P (&p)[RT], f32x4 (&o)[RT][EPL]) {
-#pragma unroll
-    for (int dt = 0; dt < EPL; ++dt) {
-      const uint32_t sel = (dt & 1) ? 0x07060302u : 0x05040100u;  // the high or low halves of two words
-      uint4 a;
-      a.x = __builtin_amdgcn_perm(word(v[1], dt >> 1), word(v[0], dt >> 1), sel);
-      a.y = __builtin_amdgcn_perm(word(v[3], dt >> 1), word(v[2], dt >> 1), sel);
-      a.z = __builtin_amdgcn_perm(word(v[5], dt >> 1), word(v[4], dt >> 1), sel);
-      a.w = __builtin_amdgcn_perm(word(v[7], dt >> 1), word(v[6], dt >> 1), sel);
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-        o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), p[rt].v, o[rt][dt], 0, 0, 0);
-    }
-  }
-  // Whether a V row's values are all finite; and value dt of it.
-  static __device__ __forceinline__ bool odd(const VRow& v) {
-    bool any = false;
-#pragma unroll
-    for (int w = 0; w < EPL / 2; ++w) {
-      const uint32_t u = word(v, w);
-      any = any || (u & 0x7f80u) == 0x7f80u || (u & 0x7f800000u) == 0x7f800000u;
-    }
-    return any;
-  }
-  static __device__ __forceinline__ void clear(VRow& v) {
-    if constexpr (EPL == 8)
-      v = make_uint4(0, 0, 0, 0);
-    else
-      v = make_uint2(0, 0);
-  }
-  static __device__ __forceinline__ float p_of(const P& p, int e) { return (float)p.v[e]; }
-  static __device__ __forceinline__ void store(uint16_t* o, const float (&f)[4 * EPL]) {
-#pragma unroll
-    for (int i = 0; i < 4 * EPL; i += 8) {
-      float g[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) g[j] = f[i + j];
-      *reinterpret_cast<uint4*>(o + i) = pack_bf16x8(g);
-    }
-  }
-};
-
-// float32
-template <int D>
-struct RowOps<float, D> {
-  static constexpr int NK = D / 16, EPL = D / 16;
-  struct K {
-    f32x4 v[NK];
-  };
-  struct VRow {
-    f32x4 v[EPL / 4];
-  };
-  struct Q {
-    f32x4 v[NK];
-  };
-  static __device__ __forceinline__ void load_q(Q& q, const float* row, int lq) {
-#pragma unroll
-    for (int c = 0; c < NK; ++c) q.v[c] = *reinterpret_cast<const f32x4*>(row + 16 * c + 4 * lq);
-  }
-  static __device__ __forceinline__ void sign_q(Q& q, float sign) {
-#pragma unroll
-    for (int c = 0; c < NK; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) q.v[c][i] = sign == 0.f ? 0.f : q.v[c][i] * sign;
-  }
-  static __device__ __forceinline__ void load_k(K& k, __amdgpu_buffer_rsrc_t r, uint32_t off, int lq) {
-#pragma unroll
-    for (int c = 0; c < NK; ++c) k.v[c] = __builtin_bit_cast(f32x4, buf_load16(r, off + 64 * c + 16 * lq));
-  }
-  static __device__ __forceinline__ void load_v(VRow& v, __amdgpu_buffer_rsrc_t r, uint32_t off) {
-#pragma unroll
-    for (int i = 0; i < EPL / 4; ++i) v.v[i] = __builtin_bit_cast(f32x4, buf_load16(r, off + 16 * i));
-  }
-  static __device__ __forceinline__ f32x4 qk(const K& k, const Q& q, f32x4 s) {
-#pragma unroll
-    for (int c = 0; c < NK; ++c)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.v[c][i], q.v[c][i], s, 0, 0, 0);
-    return s;
-  }
-  struct P {
-    float v[8];
-  };
-  static __device__ __forceinline__ float exponentiate(const f32x4 (&s)[2], float c2, P& p) {
-    float sum = 0.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        p.v[4 * h + i] = fast_exp2(s[h][i] * c2);
-        sum += p.v[4 * h + i];
-      }
-    return sum;
-  }
-  template <int RT>
-  static __device__ __forceinline__ void pv(const VRow (&v)[8], const P (&p)[RT], f32x4 (&o)[RT][EPL]) {
-#pragma unroll
-    for (int dt = 0; dt < EPL; ++dt)
-#pragma unroll
-      for (int e = 0; e < 8; ++e)
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-          o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e].v[dt / 4][dt % 4], p[rt].v[e], o[rt][dt], 0, 0, 0);
-  }
-  static __device__ __forceinline__ bool odd(const VRow& v) {
-    bool any = false;
-#pragma unroll
-    for (int i = 0; i < EPL; ++i) any = any || (__float_as_uint(v.v[i / 4][i % 4]) & 0x7f800000u) == 0x7f800000u;
-    return any;
-  }
-  static __device__ __forceinline__ void clear(VRow& v) {
-#pragma unroll
-    for (int i = 0; i < EPL / 4; ++i) v.v[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  static __device__ __forceinline__ float p_of(const P& p, int e) { return p.v[e]; }
-  static __device__ __forceinline__ void store(float* o, const float (&f)[4 * EPL]) {
-#pragma unroll
-    for (int i = 0; i < 4 * EPL; i += 4) *reinterpret_cast<f32x4*>(o + i) = f32x4{f[i], f[i + 1], f[i + 2], f[i + 3]};
-  }
-};
-
 template <typename T, int D, int RT>
 __global__ __launch_bounds__(kRowWaves * 64, sizeof(T) == 4 && D == 128 ? 1 : 2) void paged_rows_kernel(
     const T* __restrict__ Q, const T* __restrict__ K, const T* __restrict__ V, T* __restrict__ O, PagedBatch pb, int hq,
-    int hkv, int G, PagedStrides st, float c2, float sign, int causal, int max_new, int most_rows, int chunk, int chunks, float* __restrict__ part) {
-  using R = RowOps<T, D>;
-  constexpr int EPL = R::EPL;
-  constexpr int MS = 2 + 4 * EPL;  // floats per lane and row tile that the waves exchange
-  __shared__ float join[(kRowWaves - 1) * RT * MS * 64];
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63;
-  const int r = lane & 15, lq = lane >> 4;
-  // Workgroups go to the eight XCDs in turn: with the kv head innermost an XCD's L2 holds the rows of one or a few
-  // heads, which sequences that share pages (beams of one prompt) read at about the same time.
-  const int hk = blockIdx.x % hkv, split = blockIdx.z;
-  const Tile t = find_tile(pb, blockIdx.x / hkv, G, 16 * RT, max_new, 0, most_rows);
-  if (t.b < 0) return;
-  // the keys that the tile's last row sees bound the tile's
-  const int last = min(t.row0 + 16 * RT, t.rows) - 1;
-  const int end = seen_by(t, last / G, causal, pb.max_len);
-  const int k0 = split * chunk, k1 = min(end, k0 + chunk);
-  if (split > 0 && k0 >= end) return;  // (the first chunk of a tile without keys stores zeros)
-
-  typename R::Q q[RT];
-  int sees[RT];  // keys that this lane's packed row sees
-  int64_t at[RT];
-  bool there[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    const int xr = t.row0 + 16 * rt + r, x = min(xr, t.rows - 1), j = x / G, h = hk * G + x - j * G;
-    there[rt] = xr < t.rows;  // (a row that is not there reads the last one's query, and leaves nothing)
-    sees[rt] = there[rt] ? seen_by(t, j, causal, pb.max_len) : 0;
-    at[rt] = (int64_t)(t.t0 + j) * hq + h;
-    R::load_q(q[rt], Q + (int64_t)(t.t0 + j) * st.qt + (int64_t)h * st.qh, lq);
-  }
-  const int first_sees = seen_by(t, t.row0 / G, causal, pb.max_len);  // the fewest keys that a row of the tile sees
-
-  f32x4 o[RT][EPL];
-  float m[RT], l[RT];
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    m[rt] = there[rt] ? -INFINITY : 0.f;  // (a row that is not there never asks for a raise)
-    l[rt] = 0.f;
-#pragma unroll
-    for (int dt = 0; dt < EPL; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const int32_t* table = pb.table + t.b * pb.table_stride;
-  const int page_mask = (1 << pb.page_log) - 1;
-  typename R::K kr[2];
-  typename R::VRow vr[8];
-  bool held[2];
-  // Page ids of the wave's next 32 blocks, one half per lane (-1: none, or behind `end`): one load ahead of
-  // the rows' own, which wait for nothing then.
-  int ids = -1;
-  auto load_ids = [&](int kb) {
-    const int key = kb + 32 * kRowWaves * (lane >> 1) + 16 * (lane & 1);
-    ids = key < min(pb.max_len, k0 + chunk) ? table[key >> pb.page_log] : -1;
-  };
-  // Half h of the wave's block n (at key kb): its page's rows as far as keys below `end` go; a half in no
-  // page, or behind `end`, reads as zeros.
-  auto rsrc = [&](const T* base, int64_t sp, int64_t sh, int64_t sr, int kb, int n, int h, bool* in) {
-    const int key = kb + 16 * h;
-    const int id = __builtin_amdgcn_readlane(ids, 2 * (n & 31) + h);
-    const bool ok = pb.is_page(id);
-    *in = ok;
-    const int rows = ok ? min(16, end - key) : 0;
-    const T* p = base + (int64_t)(ok ? id : 0) * sp + (int64_t)hk * sh + (int64_t)(key & page_mask) * sr;
-    return make_rsrc(p, rows > 0 ? (uint32_t)(((int64_t)(rows - 1) * sr + D) * sizeof(T)) : 0u);
-  };
-  auto load_k = [&](int kb, int n) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const auto rk = rsrc(K, st.kp, st.kh, st.kr, kb, n, h, &held[h]);
-      R::load_k(kr[h], rk, (uint32_t)(r * st.kr * sizeof(T)), lq);
-    }
-  };
-  auto load_v = [&](int kb, int n) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bool in;
-      const auto rv = rsrc(V, st.vp, st.vh, st.vr, kb, n, h, &in);
-#pragma unroll
-      for (int i = 0; i < 4; ++i)
-        R::load_v(vr[4 * h + i], rv, (uint32_t)(((4 * lq + i) * st.vr + EPL * r) * sizeof(T)));
-    }
-  };
-  int kb = k0 + 32 * wave;
-  load_ids(kb);
-  if (kb < k1) {
-    load_k(kb, 0);
-    load_v(kb, 0);
-  }
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) R::sign_q(q[rt], there[rt] ? sign : 0.f);
-#pragma unroll 1
-  for (int n = 1; kb < k1; kb += 32 * kRowWaves, ++n) {
-    f32x4 s[RT][2];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      const float mn = m[rt] == -INFINITY ? 0.f : -m[rt];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s[rt][h] = R::qk(kr[h], q[rt], f32x4{mn, mn, mn, mn});
-    }
-    const bool hole0 = !held[0], hole1 = !held[1];
-    const bool more = kb + 32 * kRowWaves < k1;
-    if (more) {
-      if ((n & 31) == 0) load_ids(kb + 32 * kRowWaves);
-      load_k(kb + 32 * kRowWaves, n);
-    }
-    const bool cut = kb + 32 > first_sees;  // some row of the tile does not see all 32 keys
-    if (cut || hole0 || hole1)
-#pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i)
-            if (kb + 16 * h + 4 * lq + i >= sees[rt] || (h == 0 ? hole0 : hole1)) s[rt][h][i] = -INFINITY;
-    typename R::P p[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float ps = R::exponentiate(s[rt], c2, p[rt]);
-      if (__any(m[rt] == -INFINITY || !(ps <= kSumMax))) {
-        // raise the rows' reference to their maximum over the block: lanes r, r + 16, .. hold one row
-        float mx = -INFINITY;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) mx = fmaxf(mx, s[rt][h][i]);
-        mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-        mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-        float d, alpha;
-        if (m[rt] == -INFINITY) {
-          d = mx == -INFINITY ? 0.f : mx;
-          alpha = 0.f;
-          m[rt] = mx;
-        } else {
-          d = fmaxf(mx, 0.f);
-          alpha = fast_exp2(-d * c2);
-          m[rt] += d;
-        }
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) s[rt][h][i] -= d;
-        l[rt] *= alpha;
-#pragma unroll
-        for (int dt = 0; dt < EPL; ++dt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) o[rt][dt][i] *= alpha;
-        ps = R::exponentiate(s[rt], c2, p[rt]);
-      }
-      l[rt] += ps;
-    }
-    if (cut) {
-      // A row that some packed rows see and others do not may hold infinities or NaN, and 0 times those is
-      // not 0: such V rows are taken out of the products and added key by key to the rows that see them.
-      bool any = false;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) any = any || R::odd(vr[e]);
-      if (__any(any)) {
-        for (int e = 0; e < 8; ++e)
-          for (int qq = 0; qq < 4; ++qq) {
-            const int key = kb + 16 * (e >> 2) + 4 * qq + (e & 3);
-            if (key >= end) continue;
-            const int id = table[key >> pb.page_log];
-            if (!pb.is_page(id)) continue;
-            const T* v = V + (int64_t)id * st.vp + (int64_t)hk * st.vh + (int64_t)(key & page_mask) * st.vr;
-            bool bad = false;
-            for (int d = lane; d < D; d += 64) bad = bad || !(fabsf(Elem<T>::load(v, d)) < INFINITY);
-            if (!__any(bad)) continue;
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-              float pe = 0.f;
-#pragma unroll
-              for (int ee = 0; ee < 8; ++ee)
-                if (ee == e) pe = R::p_of(p[rt], ee);
-              pe = __shfl(pe, 16 * qq + r, 64);
-              if (key < sees[rt])
-#pragma unroll
-                for (int dt = 0; dt < EPL; ++dt)
-#pragma unroll
-                  for (int i = 0; i < 4; ++i) o[rt][dt][i] += pe * Elem<T>::load(v, EPL * (4 * lq + i) + dt);
-            }
-#pragma unroll
-            for (int ee = 0; ee < 8; ++ee)
-              if (ee == e && lq == qq) R::clear(vr[ee]);
-          }
-      }
-    }
-    R::template pv<RT>(vr, p, o);
-    if (more) load_v(kb + 32 * kRowWaves, n);
-  }
-
-  // Join the waves in wave order.
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    l[rt] += __shfl_xor(l[rt], 16, 64);
-    l[rt] += __shfl_xor(l[rt], 32, 64);
-  }
-  if (wave > 0) {
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      float* p = join + ((wave - 1) * RT + rt) * MS * 64 + lane;
-      p[0] = m[rt];
-      p[64] = l[rt];
-#pragma unroll
-      for (int dt = 0; dt < EPL; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) p[(2 + 4 * dt + i) * 64] = o[rt][dt][i];
-    }
-  }
-  __syncthreads();
-  if (wave > 0) return;
-#pragma unroll
-  for (int rt = 0; rt < RT; ++rt) {
-    float mo[kRowWaves], mt = m[rt];
-    mo[0] = m[rt];
-#pragma unroll
-    for (int w = 1; w < kRowWaves; ++w) {
-      mo[w] = join[((w - 1) * RT + rt) * MS * 64 + lane];
-      mt = fmaxf(mt, mo[w]);
-    }
-    float f[4 * EPL];  // columns 4 EPL lq ..: tile dt's column i is EPL (4 lq + i) + dt
-    const float a0 = mo[0] == -INFINITY ? 0.f : fast_exp2((mo[0] - mt) * c2);
-    float lt = l[rt] * a0;
-#pragma unroll
-    for (int dt = 0; dt < EPL; ++dt)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) f[EPL * i + dt] = o[rt][dt][i] * a0;
-#pragma unroll
-    for (int w = 1; w < kRowWaves; ++w) {
-      const float* p = join + ((w - 1) * RT + rt) * MS * 64 + lane;
-      const float a = mo[w] == -INFINITY ? 0.f : fast_exp2((mo[w] - mt) * c2);
-      lt += a * p[64];
-#pragma unroll
-      for (int dt = 0; dt < EPL; ++dt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) f[EPL * i + dt] += a * p[(2 + 4 * dt + i) * 64];
-    }
-    if (!there[rt]) continue;
-    if (part == nullptr) {
-      const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
-#pragma unroll
-      for (int i = 0; i < 4 * EPL; ++i) f[i] *= inv;
-      const int64_t tok = at[rt] / hq, h = at[rt] - tok * hq;
-      R::store(O + tok * st.ot + h * st.oh + 4 * EPL * lq, f);
-    } else {
-      float* po = part_o<D>(part, at[rt], chunks, split) + 4 * EPL * lq;
-#pragma unroll
-      for (int i = 0; i < 4 * EPL; i += 4) *reinterpret_cast<f32x4*>(po + i) = f32x4{f[i], f[i + 1], f[i + 2], f[i + 3]};
-      if (lq == 0) part_ml<D>(part, (int64_t)pb.tokens * hq, chunks, at[rt])[split] = make_float2(mt, lt);
-    }
-  }
+    int hkv, int G, PagedStrides st, float c2, float sign, int causal, int max_new, int most_rows, int chunk, int chunks,
+    float* __restrict__ part) {
+  __shared__ float join[RowLds<T, D, RT>::FLOATS];
+  paged_rows<T, D, RT>(join, blockIdx.x, blockIdx.z, Q, K, V, O, pb, hq, hkv, G, st, c2, sign, causal, max_new, most_rows,
+                       chunk, chunks, part);
 }
 
 // Joins the chunks of a token's query heads, relative to each row's maximum.  Chunks hold few_chunk keys in sequences
@@ -597,68 +139,68 @@ int chunk_of(const PagedCall& c, int64_t tiles, int least, int64_t most) {
   return (int)chunk;
 }
 
-template <typename T, int D, int RT>
-void launch_rows(const PagedCall& c, int most_rows, int64_t tiles, int chunk, int used, int chunks, float* part) {
-  paged_rows_kernel<T, D, RT><<<dim3((unsigned)(tiles * c.hkv), 1, used), kRowWaves * 64, 0, stream()>>>(
-      (const T*)c.q, (const T*)c.k, (const T*)c.v, (T*)c.o, c.pb, c.hq, c.hkv, c.G, c.st, c.c2, c.sign, c.causal, c.max_new,
-      most_rows, chunk, chunks, part);
+PagedPart part_of(const PagedCall& c, int64_t tiles, int least, int64_t most) {
+  const int chunk = chunk_of(c, tiles, least, most);
+  return PagedPart{(int)(tiles * c.hkv), chunk, c.pb.max_len > chunk ? (c.pb.max_len + chunk - 1) / chunk : 1};
 }
 
-// Packed rows of a sequence up to which paged_rows_kernel takes it beside paged_tiles.hip: with 160 rows of up to 8000
-// keys (four sequences) it is at 55 us and the tiles at 80, with 96 of 2000 at 19 against 32; with 400 to 512
-// rows the tiles come level (512 of 16384 keys: 59 us against 87).
+template <typename T, int D, int RT>
+void launch_rows(const PagedCall& c, const PagedPart& p, float* part) {
+  paged_rows_kernel<T, D, RT><<<dim3(p.columns, 1, p.used), kRowWaves * 64, 0, stream()>>>(
+      (const T*)c.q, (const T*)c.k, (const T*)c.v, (T*)c.o, c.pb, c.hq, c.hkv, c.G, c.st, c.c2, c.sign, c.causal, c.max_new,
+      INT32_MAX, p.chunk, p.used, p.used > 1 ? part : nullptr);
+}
+
+// Packed rows of a sequence up to which tiles of 32 rows take it rather than those of paged_tiles.hip: with 160 rows of
+// up to 8000 keys (four sequences) they are at 55 us and the others at 80, with 96 of 2000 at 19 against 32;
+// with 400 to 512 rows the large tiles come level (512 of 16384 keys: 59 us against 87).
 constexpr int kFewRows = 256;
 
 template <typename T, int D>
 int launch(const PagedCall& c) {
   const int64_t most = (int64_t)c.max_new * c.G, cus = cu_count();
   // (the tiles take pools of equal strides only)
-  const bool tiles_too =
+  const bool many_too =
       sizeof(T) == 2 && most > kFewRows && c.st.kp == c.st.vp && c.st.kh == c.st.vh && c.st.kr == c.st.vr;
-  // rows up to which paged_rows_kernel takes a sequence; a sequence alone is one or the other's
-  const int few = tiles_too ? (c.pb.batch > 1 ? kFewRows : 0) : INT32_MAX;
-  const int rt = most <= 16 ? 1 : 2;
-  const int64_t few_tiles = few == 0 ? 0 : tiles_of(c, 16 * rt);
+  const bool few_too = !many_too || c.pb.batch > 1;  // (a sequence alone is one or the other's)
   // Tiles of 256 rows read K and V half as often as those of 128, of which a CU holds two: better where one
   // workgroup per CU is all there is and its keys are many (2048 tokens of 16384, 16 / 8 heads: 281 us against
   // 317), worse with ragged or short ones (four chunks of 512 of 8192: 196 against 179).
-  const int64_t tiles8 = tiles_too ? tiles_of(c, 256) : 0;
-  const int waves = tiles8 * c.hkv <= cus && c.pb.max_len >= 6144 ? 8 : 4;
-  const int64_t many_tiles = !tiles_too ? 0 : (waves == 8 ? tiles8 : tiles_of(c, 128));
-  // Chunks of keys: more workgroups than the chip holds at once, and shorter chunks than 512 keys of a tile, cost
-  // more in partials than they gain (2600 keys of six ragged chunks: 88 us, 98 in twice as many chunks).  The
-  // rows kernel runs two workgroups per CU, one of fp32 at d 128.
-  const int few_chunk = chunk_of(c, few_tiles, 128, 5 * cus * (sizeof(T) == 4 && D == 128 ? 1 : 2) / 4);
-  const int many_chunk = chunk_of(c, many_tiles, 512, waves == 8 ? cus : 2 * cus);
-  auto count = [&](int chunk) { return c.pb.max_len > chunk ? (c.pb.max_len + chunk - 1) / chunk : 1; };
-  const int few_chunks = few ? count(few_chunk) : 1, many_chunks = tiles_too ? count(many_chunk) : 1;
+  const int64_t tiles8 = many_too && !few_too ? tiles_of(c, 256) : 0;
+  const int waves = tiles8 > 0 && tiles8 * c.hkv <= cus && c.pb.max_len >= 6144 ? 8 : 4;
+  const int rt = most <= 16 ? 1 : 2;
+  const int64_t few_tiles = few_too ? tiles_of(c, 16 * rt) : 0;
+  const int64_t many_tiles = !many_too ? 0 : (waves == 8 ? tiles8 : tiles_of(c, 128));
+  KH_REQUIRE((few_tiles + many_tiles) * c.hkv <= (1 << 28) && (int64_t)c.pb.tokens * c.hq <= INT32_MAX,
+             "kh_paged_attention: too many query rows");
+  // Chunks of keys: up to one and a half times the workgroups that the chip holds at once (their tile counts are upper
+  // bounds; 2048 of 16384 keys: 273 us, 291 with up to as many as it holds, 288 with twice as many), and 512
+  // keys of a tile at least: partials cost more than shorter chunks gain.  The chip holds two workgroups of the
+  // rows kernel per CU, one of fp32 at d 128, and here a quarter more is best.
+  const PagedPart few = part_of(c, few_tiles, 128, 5 * cus * (sizeof(T) == 4 && D == 128 ? 1 : 2) / 4);
+  const PagedPart many = part_of(c, many_tiles, 512, 3 * cus * (waves == 8 ? 1 : 2) / 2);
+  const int few_chunks = few_too ? few.used : 1, many_chunks = many_too ? many.used : 1;
   const int chunks = few_chunks > many_chunks ? few_chunks : many_chunks;
-  KH_REQUIRE(few_tiles * c.hkv <= INT32_MAX && many_tiles * c.hkv <= INT32_MAX && chunks <= 65535,
-             "kh_paged_attention: too many tiles");
-  KH_REQUIRE((int64_t)c.pb.tokens * c.hq <= INT32_MAX, "kh_paged_attention: too many rows");
+  KH_REQUIRE(chunks <= 65535 && (int64_t)few.columns * few_chunks + (int64_t)many.columns * many_chunks <= INT32_MAX,
+             "kh_paged_attention: too many chunks of keys");
   float* part = nullptr;
   const int64_t rows = (int64_t)c.pb.tokens * c.hq;
   if (chunks > 1) {
     part = (float*)scratch_alloc((size_t)rows * chunks * (D + 2) * 4);
     if (part == nullptr) return KH_ERR_OOM;
   }
-  hipError_t e = hipSuccess;
-  if (tiles_too) {
-    launch_paged_tiles(c, D, waves, few, many_tiles, many_chunk, many_chunks, chunks,
-                       many_chunks > 1 ? part : nullptr);
-    e = hipGetLastError();
-  }
-  if (few && e == hipSuccess) {
-    float* p = few_chunks > 1 ? part : nullptr;
-    if (rt == 1)
-      launch_rows<T, D, 1>(c, few, few_tiles, few_chunk, few_chunks, chunks, p);
-    else
-      launch_rows<T, D, 2>(c, few, few_tiles, few_chunk, few_chunks, chunks, p);
-    e = hipGetLastError();
-  }
+  if (many_too && few_too)
+    launch_paged_mixed(c, D, kFewRows, many, few, chunks, part);
+  else if (many_too)
+    launch_paged_tiles(c, D, waves, many, chunks, part);
+  else if (rt == 1)
+    launch_rows<T, D, 1>(c, few, part);
+  else
+    launch_rows<T, D, 2>(c, few, part);
+  hipError_t e = hipGetLastError();
   if (part && e == hipSuccess) {
-    const MergeArgs a{c.hq,      c.causal, c.max_new, c.G, few, few_chunks > 1 ? few_chunk : 0, many_chunks > 1 ? many_chunk : 0,
-                      chunks};
+    const MergeArgs a{c.hq, c.causal, c.max_new, c.G, !many_too ? INT32_MAX : (few_too ? kFewRows : 0),
+                      few_chunks > 1 ? few.chunk : 0, many_chunks > 1 ? many.chunk : 0, chunks};
     if (c.pb.tokens >= cu_count())
       paged_merge_kernel<T, D><<<c.pb.tokens, 256, 0, stream()>>>(part, (T*)c.o, c.pb, c.st, c.c2, a);
     else

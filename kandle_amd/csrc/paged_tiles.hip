@@ -11,8 +11,7 @@
 // read inside one such block, so a block's place is a lane's value read as scalars (one lane per block, worked
 // out for 1024 keys at once), and its buffer range ends with the page's rows that the tile sees (others, and
 // blocks in no page, read as zeros).  K and V pools have equal strides here.
-#include "flash_tiles.h"
-#include "paged.h"
+#include "paged_rows.h"
 
 using namespace kh;
 
@@ -32,18 +31,20 @@ struct TileCfg {
   static_assert(NK >= 1 && BN % 64 == 0 && THREADS / CPR % 16 == 0, "whole 16-key blocks per load");
 };
 
-template <int D, int WAVES, int BN, int MINB>
-__global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
-    const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K, const uint16_t* __restrict__ V,
-    uint16_t* __restrict__ O, PagedBatch pb, int hq, int hkv, int G, PagedStrides st, float c2, float sign, int causal,
-    int max_new, int min_rows, int chunk, int chunks, float* __restrict__ part) {
+// Tile `column` / hkv of kv head `column` % hkv (innermost: an XCD's L2 holds few heads) and chunk `split`; smem: 2
+// STAGE elements of LDS, odd: whether a wave's V pieces of a staged tile held infinities or NaN.
+template <int D, int WAVES, int BN>
+__device__ __forceinline__ void paged_tiles(uint16_t* smem, int (&odd)[2][WAVES], int column, int split,
+                                            const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K,
+                                            const uint16_t* __restrict__ V, uint16_t* __restrict__ O,
+                                            const PagedBatch& pb, int hq, int hkv, int G, const PagedStrides& st, float c2,
+                                            float sign, int causal, int max_new, int min_rows, int chunk, int chunks,
+                                            float* __restrict__ part) {
   using C = TileCfg<D, WAVES, BN>;
-  __shared__ __attribute__((aligned(16))) uint16_t smem[2 * C::STAGE];
-  __shared__ int odd[2][WAVES];  // whether a wave's V pieces of a tile held infinities or NaN
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int r = lane & 31, g = lane >> 5;
-  const int hk = blockIdx.x % hkv, split = blockIdx.z;  // the kv head innermost: an XCD's L2 holds few heads
-  const Tile t = find_tile(pb, blockIdx.x / hkv, G, 32 * WAVES, max_new, min_rows, INT32_MAX);
+  const int hk = column % hkv;
+  const Tile t = find_tile(pb, column / hkv, G, 32 * WAVES, max_new, min_rows, INT32_MAX);
   if (t.b < 0) return;
   const int end = seen_by(t, (min(t.row0 + 32 * WAVES, t.rows) - 1) / G, causal, pb.max_len);
   const int k0 = split * chunk, k1 = min(end, k0 + chunk);
@@ -301,29 +302,76 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
 }
 
 template <int D, int WAVES, int BN, int MINB>
-void launch_tiles(const PagedCall& c, int min_rows, int64_t tiles, int chunk, int used, int chunks, float* part) {
-  paged_tiles_kernel<D, WAVES, BN, MINB><<<dim3((unsigned)(tiles * c.hkv), 1, used), WAVES * 64, 0, stream()>>>(
+__global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
+    const uint16_t* __restrict__ Q, const uint16_t* __restrict__ K, const uint16_t* __restrict__ V,
+    uint16_t* __restrict__ O, PagedBatch pb, int hq, int hkv, int G, PagedStrides st, float c2, float sign, int causal,
+    int max_new, int min_rows, int chunk, int chunks, float* __restrict__ part) {
+  __shared__ __attribute__((aligned(16))) uint16_t smem[2 * TileCfg<D, WAVES, BN>::STAGE];
+  __shared__ int odd[2][WAVES];
+  paged_tiles<D, WAVES, BN>(smem, odd, blockIdx.x, blockIdx.z, Q, K, V, O, pb, hq, hkv, G, st, c2, sign, causal, max_new,
+                            min_rows, chunk, chunks, part);
+}
+
+// Sequences of many rows and of few (chunks of prompts beside single tokens) in one launch, so that they run beside
+// each other: the first many.columns * many.used workgroups take tiles of 128 rows, the others of 32.  As two
+// launches one after the other six ragged chunks of up to 300 tokens took 88 us, four of 512 of 8192 179;
+// together 70 and 113.
+template <int D>
+__global__ __launch_bounds__(256, 2) void paged_mixed_kernel(const uint16_t* __restrict__ Q,
+                                                             const uint16_t* __restrict__ K,
+                                                             const uint16_t* __restrict__ V, uint16_t* __restrict__ O,
+                                                             PagedBatch pb, int hq, int hkv, int G, PagedStrides st,
+                                                             float c2, float sign, int causal, int max_new, int few_rows,
+                                                             PagedPart many, PagedPart few, int chunks,
+                                                             float* __restrict__ part) {
+  constexpr int TILE = 4 * TileCfg<D, 4, 64>::STAGE, ROWS = 4 * RowLds<uint16_t, D, 2>::FLOATS;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[TILE > ROWS ? TILE : ROWS];
+  __shared__ int odd[2][4];
+  const int x = blockIdx.x, first = many.columns * many.used;
+  if (x < first)
+    paged_tiles<D, 4, 64>(reinterpret_cast<uint16_t*>(lds), odd, x % many.columns, x / many.columns, Q, K, V, O, pb, hq, hkv,
+                          G, st, c2, sign, causal, max_new, few_rows, many.chunk, chunks, many.used > 1 ? part : nullptr);
+  else
+    paged_rows<uint16_t, D, 2>(reinterpret_cast<float*>(lds), (x - first) % few.columns, (x - first) / few.columns, Q, K, V,
+                               O, pb, hq, hkv, G, st, c2, sign, causal, max_new, few_rows, few.chunk, chunks,
+                               few.used > 1 ? part : nullptr);
+}
+
+template <int D, int WAVES, int BN, int MINB>
+void launch_tiles(const PagedCall& c, const PagedPart& many, int chunks, float* part) {
+  paged_tiles_kernel<D, WAVES, BN, MINB><<<dim3(many.columns, 1, many.used), WAVES * 64, 0, stream()>>>(
       (const uint16_t*)c.q, (const uint16_t*)c.k, (const uint16_t*)c.v, (uint16_t*)c.o, c.pb, c.hq, c.hkv, c.G, c.st, c.c2,
-      c.sign, c.causal, c.max_new, min_rows, chunk, chunks, part);
+      c.sign, c.causal, c.max_new, 0, many.chunk, chunks, many.used > 1 ? part : nullptr);
+}
+
+template <int D>
+void launch_mixed(const PagedCall& c, int few_rows, const PagedPart& many, const PagedPart& few, int chunks, float* part) {
+  paged_mixed_kernel<D><<<(unsigned)(many.columns * many.used + few.columns * few.used), 256, 0, stream()>>>(
+      (const uint16_t*)c.q, (const uint16_t*)c.k, (const uint16_t*)c.v, (uint16_t*)c.o, c.pb, c.hq, c.hkv, c.G, c.st, c.c2,
+      c.sign, c.causal, c.max_new, few_rows, many, few, chunks, part);
 }
 
 }  // namespace
 
 namespace kh {
 
-void launch_paged_tiles(const PagedCall& c, int d, int waves, int min_rows, int64_t tiles, int chunk, int used,
-                        int chunks, float* part) {
-  if (d == 128) {
-    if (waves == 8)
-      launch_tiles<128, 8, 128, 1>(c, min_rows, tiles, chunk, used, chunks, part);
-    else
-      launch_tiles<128, 4, 64, 2>(c, min_rows, tiles, chunk, used, chunks, part);
-  } else {
-    if (waves == 8)
-      launch_tiles<64, 8, 128, 1>(c, min_rows, tiles, chunk, used, chunks, part);
-    else
-      launch_tiles<64, 4, 64, 2>(c, min_rows, tiles, chunk, used, chunks, part);
-  }
+void launch_paged_tiles(const PagedCall& c, int d, int waves, const PagedPart& many, int chunks, float* part) {
+  if (d == 128 && waves == 8)
+    launch_tiles<128, 8, 128, 1>(c, many, chunks, part);
+  else if (d == 128)
+    launch_tiles<128, 4, 64, 2>(c, many, chunks, part);
+  else if (waves == 8)
+    launch_tiles<64, 8, 128, 1>(c, many, chunks, part);
+  else
+    launch_tiles<64, 4, 64, 2>(c, many, chunks, part);
+}
+
+void launch_paged_mixed(const PagedCall& c, int d, int few_rows, const PagedPart& many, const PagedPart& few, int chunks,
+                        float* part) {
+  if (d == 128)
+    launch_mixed<128>(c, few_rows, many, few, chunks, part);
+  else
+    launch_mixed<64>(c, few_rows, many, few, chunks, part);
 }
 
 }  // namespace kh
