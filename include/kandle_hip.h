@@ -504,7 +504,8 @@ int kh_gemv_swiglu(int prologue, const void* x, const void* norm_w, float eps, c
 
 /* A cache in pages: pools k_pages / v_pages [num_pages, hkv, page_size, d] (strides below, the d axis
  * contiguous; page_size a power of two from 16 to 4096), a page table [batch, table_width] of device
- * int32 page ids (row stride table_stride; an id outside [0, num_pages), by convention -1, is no page)
+ * int32 page ids (row stride table_stride; an id outside [0, num_pages), by convention -1, is no page;
+ * table_width * page_size up to 2^30, batch up to 65535)
  * and kv_lens [batch] (device int32): how many rows each sequence has cached, this call's new tokens
  * among them.  Row p of sequence b lies in page page_table[b][p / page_size] at p % page_size.  The new
  * tokens of all sequences are packed: sequence b's are rows query_starts[b] .. query_starts[b + 1] - 1

@@ -60,7 +60,7 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& pb, int x, int G, in
     const int per = (G + rows - 1) / rows;
     t.b = x / per;
     at = x - t.b * per;
-    if (t.b >= pb.batch) t.b = -1;
+    if (t.b >= pb.batch || G <= above || G > upto) t.b = -1;
   } else {
     const int lane = threadIdx.x & 63;
     for (int b0 = 0; b0 < pb.batch; b0 += 64) {

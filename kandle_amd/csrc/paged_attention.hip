@@ -228,8 +228,8 @@ int paged_batch(const char* who, const int32_t* table, const int32_t* lens, cons
   KH_REQUIRE(tokens >= 0 && tokens <= INT32_MAX && batch >= 0 && batch <= 65535, "%s: bad token or sequence count", who);
   KH_REQUIRE(num_pages >= 0 && num_pages <= INT32_MAX && table_width >= 0 && table_stride >= table_width,
              "%s: bad page table", who);
-  KH_REQUIRE(table_width * page_size <= INT32_MAX, "%s: a page table of %lld pages of %lld rows passes 2^31 rows", who,
-             (long long)table_width, (long long)page_size);
+  KH_REQUIRE(table_width <= (1 << 30) && table_width * page_size <= (1 << 30),
+             "%s: a page table of %lld pages of %lld rows passes 2^30 rows", who, (long long)table_width, (long long)page_size);
   KH_REQUIRE(starts != nullptr || tokens == batch, "%s: without query starts every sequence has one token (%lld tokens, "
              "%lld sequences)", who, (long long)tokens, (long long)batch);
   KH_REQUIRE(max_kv_len >= 0, "%s: negative max_kv_len", who);

@@ -400,7 +400,7 @@ int kh_pages_reserve(int32_t* page_table, int64_t table_stride, int32_t* kv_lens
   KH_REQUIRE(rows <= kMaxRows, "kh_pages_reserve: %lld rows, at most %d", (long long)rows, kMaxRows);
   KH_REQUIRE(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
              "kh_pages_reserve: page size %lld is not a power of two from 16 to 4096", (long long)page_size);
-  KH_REQUIRE(table_width * page_size <= INT32_MAX, "kh_pages_reserve: the page table passes 2^31 rows");
+  KH_REQUIRE(table_width * page_size <= (1 << 30), "kh_pages_reserve: the page table passes 2^30 rows");
   KH_REQUIRE(info && (rows == 0 || (kv_lens && counts && moves)) && (rows == 0 || table_width == 0 || page_table) &&
                  (num_pages == 0 || page_refs),
              "kh_pages_reserve: null pointer");

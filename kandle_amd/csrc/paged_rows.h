@@ -69,11 +69,16 @@ struct RowOps<uint16_t, D> {
     else
       v = __builtin_bit_cast(uint2, __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0));
   }
-  static __device__ __forceinline__ f32x4 qk(const K& k, const Q& q, f32x4 s) {
+  // (the products of different sums take turns: one that waits for its own last result leaves the matrix core idle)
+  template <int RT>
+  static __device__ __forceinline__ void qk(const K (&k)[2], const Q (&q)[RT], f32x4 (&s)[RT][2]) {
 #pragma unroll
     for (int c = 0; c < NK; ++c)
-      s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k.v[c]), q.v[c], s, 0, 0, 0);
-    return s;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt)
+          s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, k[h].v[c]), q[rt].v[c], s[rt][h], 0, 0, 0);
   }
   static __device__ __forceinline__ uint32_t word(const VRow& v, int w) {
     if constexpr (EPL == 8)
@@ -171,12 +176,17 @@ struct RowOps<float, D> {
 #pragma unroll
     for (int i = 0; i < EPL / 4; ++i) v.v[i] = __builtin_bit_cast(f32x4, buf_load16(r, off + 16 * i));
   }
-  static __device__ __forceinline__ f32x4 qk(const K& k, const Q& q, f32x4 s) {
+  template <int RT>
+  static __device__ __forceinline__ void qk(const K (&k)[2], const Q (&q)[RT], f32x4 (&s)[RT][2]) {
 #pragma unroll
     for (int c = 0; c < NK; ++c)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) s = __builtin_amdgcn_mfma_f32_16x16x4f32(k.v[c][i], q.v[c][i], s, 0, 0, 0);
-    return s;
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt)
+            s[rt][h] = __builtin_amdgcn_mfma_f32_16x16x4f32(k[h].v[c][i], q[rt].v[c][i], s[rt][h], 0, 0, 0);
   }
   struct P {
     float v[8];
@@ -195,9 +205,9 @@ struct RowOps<float, D> {
   template <int RT>
   static __device__ __forceinline__ void pv(const VRow (&v)[8], const P (&p)[RT], f32x4 (&o)[RT][EPL]) {
 #pragma unroll
-    for (int dt = 0; dt < EPL; ++dt)
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
-      for (int e = 0; e < 8; ++e)
+      for (int dt = 0; dt < EPL; ++dt)
 #pragma unroll
         for (int rt = 0; rt < RT; ++rt)
           o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[e].v[dt / 4][dt % 4], p[rt].v[e], o[rt][dt], 0, 0, 0);
@@ -325,9 +335,9 @@ __device__ __forceinline__ void paged_rows(float* join, int column, int split, c
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
       const float mn = m[rt] == -INFINITY ? 0.f : -m[rt];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) s[rt][h] = R::qk(kr[h], q[rt], f32x4{mn, mn, mn, mn});
+      s[rt][0] = s[rt][1] = f32x4{mn, mn, mn, mn};
     }
+    R::template qk<RT>(kr, q, s);
     const bool hole0 = !held[0], hole1 = !held[1];
     const bool more = kb + 32 * kRowWaves < k1;
     if (more) {

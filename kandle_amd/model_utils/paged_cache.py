@@ -123,8 +123,11 @@ class PagedKVCache:
 
     def free(self, sequences: Sequence[int]) -> None:
         """Gives back the pages of these sequences."""
+        s = np.asarray(list(sequences), np.int64)
+        if (s < 0).any() or (s >= self.max_sequences).any():
+            raise ValueError(f"PagedKVCache: sequences outside [0, {self.max_sequences})")
         parents = np.arange(self.max_sequences)
-        parents[np.asarray(sequences, np.int64)] = -1
+        parents[s] = -1
         self.fork(parents)
 
     def reset(self) -> None:

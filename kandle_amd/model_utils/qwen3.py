@@ -505,7 +505,9 @@ class Qwen3ForCausalLM:
         whatever else they have in common.  Selection, the beams' page bookkeeping and the forward of a step run on
         the device; with use_graph they are captured (two steps: the page tables change places) and replayed, and
         the host reads a step's tokens and parents back to follow them."""
-        prompts = [np.asarray(p, np.int32).reshape(-1) for p in prompts]
+        prompts = [np.asarray(p, np.int32) for p in prompts]
+        if any(p.ndim != 1 for p in prompts):
+            raise ValueError("generate_beams: a list of prompts, each a list of token ids, expected")
         G, B, N = len(prompts), int(num_beams), int(max_new_tokens)
         if not G or not all(len(p) for p in prompts) or B < 1 or N < 1:
             raise ValueError("generate_beams: prompts of one token or more, one beam or more, one new token or more expected")

@@ -61,6 +61,11 @@ def test_forked_freed_and_moved_sequences(hip):
             ids[1] = []
             live = cache.compact()             # the others' pages move to the front
             assert live == cache.num_pages - cache.free_pages() and cache.page_table.numpy().max() < live
+    for bad in ([-1], [3]):
+        with pytest.raises(ValueError, match="sequences"):
+            cache.free(bad)
+    with pytest.raises(ValueError, match="parents"):
+        cache.fork([0, 1, 3])
     cache.reset()
     assert cache.free_pages() == 24 and cache.lens.tolist() == [0, 0, 0]
     cache.dispose()
@@ -147,7 +152,7 @@ def test_beams_by_graph_are_the_eager_ones_bit_for_bit(hip):
 
 def test_beam_refusals(hip):
     cfg, model, _ = make()
-    for bad in (([], 2, 4), ([[]], 2, 4), ([[1]], 0, 4), ([[1]], 2, 0), ([[1]], 65, 4), ([[1]], 2, 256)):
+    for bad in (([], 2, 4), ([1, 2], 2, 4), ([[]], 2, 4), ([[1]], 0, 4), ([[1]], 2, 0), ([[1]], 65, 4), ([[1]], 2, 256)):
         with pytest.raises(ValueError):
             model.generate_beams(*bad)
     with pytest.raises(ValueError, match="eos"):
