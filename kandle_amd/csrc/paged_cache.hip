@@ -75,6 +75,39 @@ __global__ __launch_bounds__(256) void pages_fork_refs_kernel(const int32_t* __r
   }
 }
 
+// Both at once for small tables, by one workgroup with the counts' changes in LDS: a beam step's 64 rows of 70 pages
+// take 4.8 us instead of 2.7 + 2.6 and the gap between two launches; 256 rows of 64 would take 11.
+constexpr int kForkPages = 16384, kForkRows = 2048, kForkEntries = 8192;
+__global__ __launch_bounds__(1024) void pages_fork_small_kernel(const int32_t* __restrict__ table, int64_t stride,
+                                                                const int32_t* __restrict__ lens,
+                                                                const int32_t* __restrict__ refs,
+                                                                const int32_t* __restrict__ parents, int rows, int width,
+                                                                int num_pages, int32_t* __restrict__ new_table,
+                                                                int32_t* __restrict__ new_lens,
+                                                                int32_t* __restrict__ new_refs) {
+  __shared__ int change[kForkPages];
+  __shared__ int children[kForkRows];
+  for (int i = threadIdx.x; i < num_pages; i += 1024) change[i] = 0;
+  for (int i = threadIdx.x; i < rows; i += 1024) children[i] = 0;
+  __syncthreads();
+  for (int i = threadIdx.x; i < rows; i += 1024) {
+    const int p = parents[i];
+    const bool has = (unsigned)p < (unsigned)rows;
+    if (has) atomicAdd(children + p, 1);
+    new_lens[i] = has ? lens[p] : 0;
+  }
+  __syncthreads();
+#pragma unroll 4
+  for (int i = threadIdx.x; i < rows * width; i += 1024) {
+    const int s = i / width, c = i - s * width, p = parents[s], delta = children[s] - 1;
+    const int mine = table[s * stride + c];
+    new_table[i] = (unsigned)p < (unsigned)rows ? table[p * stride + c] : -1;
+    if (delta != 0 && (unsigned)mine < (unsigned)num_pages) atomicAdd(change + mine, delta);
+  }
+  __syncthreads();
+  for (int i = threadIdx.x; i < num_pages; i += 1024) new_refs[i] = refs[i] + change[i];
+}
+
 // ---- reserve ----------------------------------------------------------------------------------
 constexpr int kOne = 1024;      // threads of the one-workgroup kernels
 constexpr int kMaxRows = 2048;  // rows that kh_pages_reserve's LDS holds
@@ -379,6 +412,12 @@ int kh_pages_fork(const int32_t* page_table, int64_t table_stride, const int32_t
                  !shares(new_refs, num_pages, page_refs, num_pages),
              "kh_pages_fork: the results must not share memory with the inputs");
   if (rows == 0 && num_pages == 0) return KH_OK;
+  if (num_pages <= kForkPages && rows <= kForkRows && rows * table_width <= kForkEntries) {
+    pages_fork_small_kernel<<<1, 1024, 0, stream()>>>(page_table, table_stride, kv_lens, page_refs, parents, (int)rows,
+                                                      (int)table_width, (int)num_pages, new_table, new_lens, new_refs);
+    KH_CHECK_LAUNCH();
+    return KH_OK;
+  }
   int64_t n = rows * table_width;
   if (n < num_pages) n = num_pages;
   pages_fork_kernel<<<blocks_for(n), 256, 0, stream()>>>(page_table, table_stride, kv_lens, page_refs, parents, (int)rows,

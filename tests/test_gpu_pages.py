@@ -33,7 +33,7 @@ def world(seed, rows, width, pages, page):
     return r, table, lens, refs
 
 
-@pytest.mark.parametrize("rows,width,pages,page", [(1, 1, 1, 16), (4, 9, 40, 16), (70, 20, 900, 32), (300, 5, 3000, 16),
+@pytest.mark.parametrize("rows,width,pages,page", [(1, 1, 1, 16), (64, 128, 6000, 16), (64, 130, 6000, 16), (3, 4, 17000, 16), (4, 9, 40, 16), (70, 20, 900, 32), (300, 5, 3000, 16),
                                                    (1500, 3, 2500, 64), (5, 700, 9000, 16)])
 def test_fork_and_reserve(hip, rows, width, pages, page):
     r, table, lens, refs = world(rows, rows, width, pages, page)
