@@ -31,11 +31,12 @@ struct PagedBatch {
     if (!starts) return t < batch ? t : -1;
     const int lane = threadIdx.x & 63;
     int below = 0;  // starts at or before t
-    for (int b0 = 0; b0 < batch; b0 += 64) {
-      const bool at = b0 + lane < batch && starts[b0 + lane] <= t;
-      const int n = __popcll(__ballot(at));
+    for (int b0 = 0; b0 < batch; b0 += 256) {
+      int n = 0;
+#pragma unroll
+      for (int k = 0; k < 256; k += 64) n += __popcll(__ballot(b0 + k + lane < batch && starts[min(b0 + k + lane, batch)] <= t));
       below += n;
-      if (n < 64) break;
+      if (n < 256) break;
     }
     const int b = below - 1;
     return b >= 0 && t < first(b) + count(b) ? b : -1;
@@ -48,7 +49,8 @@ struct PagedStrides {
 
 // The (sequence, tile) of workgroup column x of a grid over tiles of `rows` packed rows: sequence b has
 // ceil(min(n_b, max_new) * G / rows) tiles, none unless above < min(n_b, max_new) * G <= upto.  Every wave of the
-// workgroup computes it for itself; b = -1: nothing to do.
+// workgroup computes it for itself, from 256 sequences at a time, four per lane: workgroups start with this, and
+// with one sequence per lane 256 ragged chunks of prompts took FIGURE us rather than FIGURE.  b = -1: nothing to do.
 struct Tile {
   int b = -1, row0 = 0, rows = 0;  // first packed row, packed rows of the sequence
   int t0 = 0, n = 0, len = 0;      // first token, new tokens, cached rows
@@ -58,37 +60,61 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& pb, int x, int G, in
   int at = x;
   if (pb.starts == nullptr) {
     const int per = (G + rows - 1) / rows;
-    t.b = x / per;
+    t.b = __builtin_amdgcn_readfirstlane(x / per);
     at = x - t.b * per;
     if (t.b >= pb.batch || G <= above || G > upto) t.b = -1;
+    if (t.b < 0) return t;
+    t.t0 = t.b;
+    t.n = 1;
+    t.len = pb.len(t.b);
   } else {
+    constexpr int PER = 4;
     const int lane = threadIdx.x & 63;
-    for (int b0 = 0; b0 < pb.batch; b0 += 64) {
-      const int b = b0 + lane;
-      const int n = b < pb.batch ? min(pb.count(b), max_new) : 0;
-      const int tiles = n * G > above && n * G <= upto ? (n * G + rows - 1) / rows : 0;
-      int inc = tiles;
+    for (int b0 = 0; b0 < pb.batch; b0 += 64 * PER) {
+      int start[PER + 1], len[PER], tiles[PER], sum = 0;
+#pragma unroll
+      for (int k = 0; k <= PER; ++k) start[k] = min(max(pb.starts[min(b0 + PER * lane + k, pb.batch)], 0), pb.tokens);
+#pragma unroll
+      for (int k = 0; k < PER; ++k) len[k] = pb.len(min(b0 + PER * lane + k, pb.batch - 1));
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        const int n = min(max(0, start[k + 1] - start[k]), max_new);
+        tiles[k] = n * G > above && n * G <= upto ? (n * G + rows - 1) / rows : 0;
+        sum += tiles[k];
+      }
+      int inc = sum;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
         const int u = __shfl_up(inc, o, 64);
         if (lane >= o) inc += u;
       }
-      const int all = __shfl(inc, 63, 64);
+      const int all = __builtin_amdgcn_readlane(inc, 63);
       if (at < all) {
         const int who = __ffsll((unsigned long long)__ballot(inc > at)) - 1;
-        at -= __shfl(inc - tiles, who, 64);
-        t.b = b0 + who;
+        int rest = at - (inc - sum), which = 0;  // in lane `who`: its sequence, and the tile there
+        bool found = false;
+#pragma unroll
+        for (int k = 0; k < PER; ++k) {
+          if (!found && rest < tiles[k]) {
+            found = true;
+            which = k;
+            t.t0 = start[k];
+            t.n = max(0, start[k + 1] - start[k]);
+            t.len = len[k];
+          }
+          if (!found) rest -= tiles[k];
+        }
+        t.b = b0 + PER * who + __builtin_amdgcn_readlane(which, who);
+        at = __builtin_amdgcn_readlane(rest, who);
+        t.t0 = __builtin_amdgcn_readlane(t.t0, who);
+        t.n = __builtin_amdgcn_readlane(t.n, who);
+        t.len = __builtin_amdgcn_readlane(t.len, who);
         break;
       }
       at -= all;
     }
+    if (t.b < 0) return t;
   }
-  t.b = __builtin_amdgcn_readfirstlane(t.b);
-  if (t.b < 0) return t;
-  at = __builtin_amdgcn_readfirstlane(at);
-  t.t0 = pb.first(t.b);
-  t.n = pb.count(t.b);
-  t.len = pb.len(t.b);
   t.row0 = at * rows;
   t.rows = min(t.n, max_new) * G;
   if (t.row0 < 0 || t.row0 >= t.rows) t.b = -1;  // (starts that overlap can claim more tiles than there are)
@@ -126,11 +152,13 @@ struct PagedCall {
   int causal, max_new;
 };
 
-// Workgroup columns that cover every tile of `rows` packed rows.
-inline int64_t tiles_of(const PagedCall& c, int rows) {
-  const int64_t per = ((int64_t)c.max_new * c.G + rows - 1) / rows;
-  const int64_t all = (int64_t)c.pb.tokens * c.G / rows + c.pb.batch;
-  return c.pb.starts == nullptr || per * c.pb.batch < all ? per * c.pb.batch : all;
+// Workgroup columns that cover every tile of `rows` packed rows of the sequences that have more than `above` and at
+// most `upto` of them: a sequence's last tile may be part of one.
+inline int64_t tiles_of(const PagedCall& c, int rows, int above = 0, int upto = INT32_MAX) {
+  const int64_t most = (int64_t)c.max_new * c.G < upto ? (int64_t)c.max_new * c.G : upto, all = (int64_t)c.pb.tokens * c.G;
+  const int64_t batch = c.pb.batch < all / (above + 1) ? c.pb.batch : all / (above + 1);
+  const int64_t per = (most + rows - 1) / rows;
+  return c.pb.starts == nullptr || per * batch < all / rows + batch ? per * batch : all / rows + batch;
 }
 
 // How a launch form covers its sequences: workgroups for `columns` (tiles x kv heads) by `used` chunks of `chunk` keys.

@@ -131,17 +131,15 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_row_kernel(const
   for (int e = 0; e < E; ++e) Elem<T>::store(O + (int64_t)tok * st.ot + (int64_t)h * st.oh, E * lane + e, o[e] * inv);
 }
 
-// The length of a chunk of keys: the shortest of least, 2 least, 4 least ... that makes no more than `most` workgroups
-// of `tiles` tiles per kv head, or the whole length.
-int chunk_of(const PagedCall& c, int64_t tiles, int least, int64_t most) {
+// A part of a launch of `tiles` tiles per kv head, of which `there` hold rows as far as can be told here: chunks of the
+// shortest of least, 2 least, 4 least ... keys that makes no more than `most` workgroups of those, and partials
+// (one per row and chunk) of no more than most_parts rows; or of the whole length.
+PagedPart part_of(const PagedCall& c, int64_t tiles, int64_t there, int least, int64_t most, int64_t most_parts) {
+  const int64_t len = c.pb.max_len, rows = (int64_t)c.pb.tokens * c.hq;
   int64_t chunk = least;
-  while (chunk < c.pb.max_len && tiles * c.hkv * ((c.pb.max_len + chunk - 1) / chunk) > most) chunk *= 2;
-  return (int)chunk;
-}
-
-PagedPart part_of(const PagedCall& c, int64_t tiles, int least, int64_t most) {
-  const int chunk = chunk_of(c, tiles, least, most);
-  return PagedPart{(int)(tiles * c.hkv), chunk, c.pb.max_len > chunk ? (c.pb.max_len + chunk - 1) / chunk : 1};
+  auto used = [&] { return (len + chunk - 1) / chunk; };
+  while (chunk < len && (there * c.hkv * used() > most || rows * used() > most_parts)) chunk *= 2;
+  return PagedPart{(int)(tiles * c.hkv), (int)chunk, len > chunk ? (int)used() : 1};
 }
 
 template <typename T, int D, int RT>
@@ -169,16 +167,26 @@ int launch(const PagedCall& c) {
   const int64_t tiles8 = many_too && !few_too ? tiles_of(c, 256) : 0;
   const int waves = tiles8 > 0 && tiles8 * c.hkv <= cus && c.pb.max_len >= 6144 ? 8 : 4;
   const int rt = most <= 16 ? 1 : 2;
-  const int64_t few_tiles = few_too ? tiles_of(c, 16 * rt) : 0;
-  const int64_t many_tiles = !many_too ? 0 : (waves == 8 ? tiles8 : tiles_of(c, 128));
+  const int64_t few_tiles = !few_too ? 0 : tiles_of(c, 16 * rt, 0, many_too ? kFewRows : INT32_MAX);
+  const int64_t many_tiles = !many_too ? 0 : (waves == 8 ? tiles8 : tiles_of(c, 128, few_too ? kFewRows : 0));
   KH_REQUIRE((few_tiles + many_tiles) * c.hkv <= (1 << 28) && (int64_t)c.pb.tokens * c.hq <= INT32_MAX,
              "kh_paged_attention: too many query rows");
+  // Where both are there, the tiles of few rows are those of a batch in which as many sequences as can be have max_new
+  // tokens: it is only the chunks' length that depends on the guess.
+  int64_t few_there = few_tiles;
+  if (many_too && few_too) {
+    const int64_t full = c.pb.tokens / c.max_new < c.pb.batch ? c.pb.tokens / c.max_new : c.pb.batch;
+    const int64_t guess = (c.pb.tokens - full * c.max_new) * c.G / 32 + c.pb.batch - full;
+    few_there = guess < few_tiles ? guess : few_tiles;
+  }
   // Chunks of keys: up to one and a half times the workgroups that the chip holds at once (their tile counts are upper
   // bounds; 2048 of 16384 keys: 273 us, 291 with up to as many as it holds, 288 with twice as many), and 512
   // keys of a tile at least: partials cost more than shorter chunks gain.  The chip holds two workgroups of the
-  // rows kernel per CU, one of fp32 at d 128, and here a quarter more is best.
-  const PagedPart few = part_of(c, few_tiles, 128, 5 * cus * (sizeof(T) == 4 && D == 128 ? 1 : 2) / 4);
-  const PagedPart many = part_of(c, many_tiles, 512, 3 * cus * (waves == 8 ? 1 : 2) / 2);
+  // rows kernel per CU, one of fp32 at d 128, and here a quarter more is best.  Beside a prompt's many rows, whose
+  // workgroups take as long, few rows need no short chunks: partials of 2^18 rows at most (FIGURE).
+  const PagedPart few = part_of(c, few_tiles, few_there, 128, 5 * cus * (sizeof(T) == 4 && D == 128 ? 1 : 2) / 4,
+                                many_too ? 1 << 18 : INT64_MAX);
+  const PagedPart many = part_of(c, many_tiles, many_tiles, 512, 3 * cus * (waves == 8 ? 1 : 2) / 2, INT64_MAX);
   const int few_chunks = few_too ? few.used : 1, many_chunks = many_too ? many.used : 1;
   const int chunks = few_chunks > many_chunks ? few_chunks : many_chunks;
   KH_REQUIRE(chunks <= 65535 && (int64_t)few.columns * few_chunks + (int64_t)many.columns * many_chunks <= INT32_MAX,
