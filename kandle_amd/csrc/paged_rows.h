@@ -252,24 +252,37 @@ __device__ __forceinline__ void paged_rows(float* join, int column, int split, c
   const int hk = column % hkv;
   const Tile t = find_tile(pb, column / hkv, G, 16 * RT, max_new, 0, most_rows);
   if (t.b < 0) return;
-  // the keys that the tile's last row sees bound the tile's
-  const int last = min(t.row0 + 16 * RT, t.rows) - 1;
-  const int end = seen_by(t, last / G, causal, pb.max_len);
-  const int k0 = split * chunk, k1 = min(end, k0 + chunk);
-  if (split > 0 && k0 >= end) return;  // (the first chunk of a tile without keys stores zeros)
-
+  // Page ids of the wave's next 32 blocks, one half per lane (-1: none, or behind the chunk): one load ahead of
+  // the rows' own, which wait for nothing then.  The first are under way beside the length's own load.
+  const int32_t* table = pb.table + t.b * pb.table_stride;
+  const int page_mask = (1 << pb.page_log) - 1, k0 = split * chunk;
+  int ids = -1;
+  auto load_ids = [&](int kb) {
+    const int key = kb + 32 * kRowWaves * (lane >> 1) + 16 * (lane & 1);
+    ids = key < min(pb.max_len, k0 + chunk) ? table[key >> pb.page_log] : -1;
+  };
+  load_ids(k0 + 32 * wave);
   typename R::Q q[RT];
-  int sees[RT];  // keys that this lane's packed row sees
+  int at_j[RT];
   int64_t at[RT];
   bool there[RT];
 #pragma unroll
   for (int rt = 0; rt < RT; ++rt) {
     const int xr = t.row0 + 16 * rt + r, x = min(xr, t.rows - 1), j = x / G, h = hk * G + x - j * G;
     there[rt] = xr < t.rows;  // (a row that is not there reads the last one's query, and leaves nothing)
-    sees[rt] = there[rt] ? seen_by(t, j, causal, pb.max_len) : 0;
+    at_j[rt] = j;
     at[rt] = (int64_t)(t.t0 + j) * hq + h;
     R::load_q(q[rt], Q + (int64_t)(t.t0 + j) * st.qt + (int64_t)h * st.qh, lq);
   }
+  // the keys that the tile's last row sees bound the tile's
+  const int last = min(t.row0 + 16 * RT, t.rows) - 1;
+  const int end = seen_by(t, last / G, causal, pb.max_len);
+  const int k1 = min(end, k0 + chunk);
+  if (split > 0 && k0 >= end) return;  // (the first chunk of a tile without keys stores zeros)
+
+  int sees[RT];  // keys that this lane's packed row sees
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) sees[rt] = there[rt] ? seen_by(t, at_j[rt], causal, pb.max_len) : 0;
   const int first_sees = seen_by(t, t.row0 / G, causal, pb.max_len);  // the fewest keys that a row of the tile sees
 
   f32x4 o[RT][EPL];
@@ -281,18 +294,9 @@ __device__ __forceinline__ void paged_rows(float* join, int column, int split, c
 #pragma unroll
     for (int dt = 0; dt < EPL; ++dt) o[rt][dt] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int32_t* table = pb.table + t.b * pb.table_stride;
-  const int page_mask = (1 << pb.page_log) - 1;
   typename R::K kr[2];
   typename R::VRow vr[8];
   bool held[2];
-  // Page ids of the wave's next 32 blocks, one half per lane (-1: none, or behind `end`): one load ahead of
-  // the rows' own, which wait for nothing then.
-  int ids = -1;
-  auto load_ids = [&](int kb) {
-    const int key = kb + 32 * kRowWaves * (lane >> 1) + 16 * (lane & 1);
-    ids = key < min(pb.max_len, k0 + chunk) ? table[key >> pb.page_log] : -1;
-  };
   // Half h of the wave's block n (at key kb): its page's rows as far as keys below `end` go; a half in no
   // page, or behind `end`, reads as zeros.
   auto rsrc = [&](const T* base, int64_t sp, int64_t sh, int64_t sr, int kb, int n, int h, bool* in) {
@@ -322,7 +326,6 @@ __device__ __forceinline__ void paged_rows(float* join, int column, int split, c
     }
   };
   int kb = k0 + 32 * wave;
-  load_ids(kb);
   if (kb < k1) {
     load_k(kb, 0);
     load_v(kb, 0);
