@@ -131,15 +131,20 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_row_kernel(const
   for (int e = 0; e < E; ++e) Elem<T>::store(O + (int64_t)tok * st.ot + (int64_t)h * st.oh, E * lane + e, o[e] * inv);
 }
 
-// A part of a launch of `tiles` tiles per kv head, of which `there` hold rows as far as can be told here: chunks of the
-// shortest of least, 2 least, 4 least ... keys that makes no more than `most` workgroups of those, and partials
-// (one per row and chunk) of no more than most_parts rows; or of the whole length.
+// A part of a launch of `tiles` tiles per kv head, of which `there` hold rows as far as can be told here: its keys in as
+// many equal chunks (multiples of 128 keys, `least` at least) as make no more than `most` workgroups with keys, and
+// partials (one per row and chunk) of no more than most_parts rows.  With f the part of the keys that the tiles do not
+// see on average, n chunks leave there (n (1 - f) + f) workgroups with keys.
 PagedPart part_of(const PagedCall& c, int64_t tiles, int64_t there, int least, int64_t most, int64_t most_parts) {
   const int64_t len = c.pb.max_len, rows = (int64_t)c.pb.tokens * c.hq;
-  int64_t chunk = least;
-  auto used = [&] { return (len + chunk - 1) / chunk; };
-  while (chunk < len && (there * c.hkv * used() > most || rows * used() > most_parts)) chunk *= 2;
-  return PagedPart{(int)(tiles * c.hkv), (int)chunk, len > chunk ? (int)used() : 1};
+  if (len <= least || there == 0) return PagedPart{(int)(tiles * c.hkv), least, 1};
+  const double f = c.causal ? 0.5 * (c.max_new < len ? c.max_new : len) / len : 0.0;
+  int64_t n = (int64_t)(((double)most / ((double)there * c.hkv) - f) / (1.0 - f));
+  if (n > most_parts / rows) n = most_parts / rows;
+  if (n < 1) n = 1;
+  int64_t chunk = ((len + n - 1) / n + 127) / 128 * 128;
+  if (chunk < least) chunk = least;
+  return PagedPart{(int)(tiles * c.hkv), (int)chunk, (int)((len + chunk - 1) / chunk)};
 }
 
 template <typename T, int D, int RT>
@@ -179,14 +184,14 @@ int launch(const PagedCall& c) {
     const int64_t guess = (c.pb.tokens - full * c.max_new) * c.G / 32 + c.pb.batch - full;
     few_there = guess < few_tiles ? guess : few_tiles;
   }
-  // Chunks of keys: up to one and a half times the workgroups that the chip holds at once (their tile counts are upper
-  // bounds; 2048 of 16384 keys: 273 us, 291 with up to as many as it holds, 288 with twice as many), and 512
-  // keys of a tile at least: partials cost more than shorter chunks gain.  The chip holds two workgroups of the
-  // rows kernel per CU, one of fp32 at d 128, and here a quarter more is best.  Beside a prompt's many rows, whose
-  // workgroups take as long, few rows need no short chunks: partials of 2^18 rows at most (FIGURE).
-  const PagedPart few = part_of(c, few_tiles, few_there, 128, 5 * cus * (sizeof(T) == 4 && D == 128 ? 1 : 2) / 4,
-                                many_too ? 1 << 18 : INT64_MAX);
-  const PagedPart many = part_of(c, many_tiles, many_tiles, 512, 3 * cus * (waves == 8 ? 1 : 2) / 2, INT64_MAX);
+  // Chunks of keys: as many workgroups as the chip holds at once (two per CU, one of 256 rows, one of the rows kernel
+  // in fp32 at d 128).  Over 32 batches of single tokens, prompts' chunks and both: 81.7 us in the geometric mean,
+  // with a quarter or a half more of them 86.3, with twice as many 88.1, with chunk lengths of powers of two 82.9.
+  // 512 keys of a tile at least: partials cost more than shorter chunks gain.  Beside a prompt's many rows, whose
+  // workgroups take as long, few rows need no short chunks: partials of 2^18 rows at most.
+  const PagedPart few =
+      part_of(c, few_tiles, few_there, 128, cus * (sizeof(T) == 4 && D == 128 ? 1 : 2), many_too ? 1 << 18 : INT64_MAX);
+  const PagedPart many = part_of(c, many_tiles, many_tiles, 512, cus * (waves == 8 ? 1 : 2), INT64_MAX);
   const int few_chunks = few_too ? few.used : 1, many_chunks = many_too ? many.used : 1;
   const int chunks = few_chunks > many_chunks ? few_chunks : many_chunks;
   KH_REQUIRE(chunks <= 65535 && (int64_t)few.columns * few_chunks + (int64_t)many.columns * many_chunks <= INT32_MAX,
