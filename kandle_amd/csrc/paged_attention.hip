@@ -137,7 +137,8 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_row_kernel(const
 // see on average, n chunks leave there (n (1 - f) + f) workgroups with keys.
 PagedPart part_of(const PagedCall& c, int64_t tiles, int64_t there, int least, int64_t most, int64_t most_parts) {
   const int64_t len = c.pb.max_len, rows = (int64_t)c.pb.tokens * c.hq;
-  if (len <= least || there == 0) return PagedPart{(int)(tiles * c.hkv), least, 1};
+  if (there < 1) there = 1;
+  if (len <= least) return PagedPart{(int)(tiles * c.hkv), least, 1};
   const double f = c.causal ? 0.5 * (c.max_new < len ? c.max_new : len) / len : 0.0;
   int64_t n = (int64_t)(((double)most / ((double)there * c.hkv) - f) / (1.0 - f));
   if (n > most_parts / rows) n = most_parts / rows;

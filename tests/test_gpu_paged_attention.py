@@ -299,6 +299,37 @@ def test_more_query_heads_than_a_tile_has_rows(hip, starts):
         check(c, 66, [3, 0, 1], 320)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("tokens,news,lens", [
+    (1024, [512, 5], [600, 3000]),               # room for two full chunks, of which one is short
+    (600, [300, 1, 0, 1], [300, 2000, 0, 1500]),
+    (520, [1, 1], [2500, 1300]),
+    (2000, [0, 200, 3], [0, 5000, 5000])])
+def test_padded_batches(hip, dtype, tokens, news, lens):
+    """The packed rows may have room for more tokens than the sequences use."""
+    c = Cache(61, dtype, lens, 2, 128, 16)
+    st = np.concatenate([[0], np.cumsum(news)])
+    q, qh = seeded(63, (tokens, 4, 128), dtype)
+    for most in (max(news), tokens // len(news), tokens):
+        out, oh = seeded(65, (tokens, 4, 128), dtype)
+        got = F.paged_attention(q, c.k, c.v, i32(c.table), i32(c.lens), i32(st), out=out, max_query_len=most,
+                                max_kv_len=max(lens)).numpy()
+        np.testing.assert_array_equal(got[st[-1]:], oh[st[-1]:])
+        if most >= max(news):
+            compare(c, qh[:st[-1]], got[:st[-1]], st)
+
+
+def test_many_sequences(hip):
+    """More sequences than are looked through at once, with gaps, lone tokens and chunks of many rows among them."""
+    r = np.random.default_rng(67)
+    news = np.where(r.random(700) < 0.3, 0, r.integers(1, 4, 700))
+    news[[0, 255, 256, 511, 512, 699]] = [1, 150, 0, 140, 2, 133]
+    lens = news + r.integers(0, 60, 700)
+    c = Cache(69, "bfloat16", lens, 1, 64, 16)
+    check(c, 71, news, 2)
+    check(c, 72, news, 2, max_query_len=150, max_kv_len=int(lens.max()))
+
+
 def test_refusals(hip):
     c = Cache(63, "float32", [40], 2, 64, 16)
     q = F.zeros((1, 4, 64))
