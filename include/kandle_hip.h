@@ -550,7 +550,7 @@ int kh_paged_kv_write(const void* k, const void* v, void* k_pages, void* v_pages
 /* Rows follow their parents: new_table[s] = page_table[parents[s]] and new_lens likewise (a parent outside
  * [0, rows): an empty row, which frees it), and new_refs counts the new table's entries.  One call forks
  * (a row with several children), reorders (beam search) and frees.  The results are contiguous and share
- * no memory with the inputs.  No page is copied: kh_pages_reserve copies a shared tail when it grows. */
+ * no memory with the inputs or each other.  No page is copied: kh_pages_reserve copies a shared tail when it grows. */
 int kh_pages_fork(const int32_t* page_table, int64_t table_stride, const int32_t* kv_lens, const int32_t* page_refs,
                   const int32_t* parents, int64_t rows, int64_t table_width, int64_t num_pages, int32_t* new_table,
                   int32_t* new_lens, int32_t* new_refs);
@@ -561,13 +561,13 @@ int kh_pages_fork(const int32_t* page_table, int64_t table_stride, const int32_t
  * order and -1 behind them (kh_pages_copy takes them as they are); of several rows that grow on one page
  * nobody else holds, the last keeps it.  info [3]: the number of moves; the pages that were missing; the
  * rows that the table is too narrow for.  If either of the last two is not 0, nothing has changed.
- * At most 2048 rows. */
+ * At most 2048 rows, 2^30 cached rows in each and 2^31 table entries; no operands share memory. */
 int kh_pages_reserve(int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int32_t* page_refs,
                      const int32_t* counts, int64_t rows, int64_t table_width, int64_t num_pages, int64_t page_size,
                      int32_t* moves, int32_t* info);
 
 /* Moves the live pages to the front of the pool: with n of them, the i-th live page at or behind n goes to
- * the i-th free page before n.  new_table and new_refs (contiguous, no memory shared with the inputs)
+ * the i-th free page before n.  new_table and new_refs (contiguous; no result shares memory with an input)
  * are the table and the counts afterwards; moves [max_moves, 2] (max_moves >= num_pages / 2) receives
  * the (from, to) pairs for kh_pages_copy, and -1 behind them; info [2]: their number, and n. */
 int kh_pages_compact(const int32_t* page_table, int64_t table_stride, const int32_t* page_refs, int64_t rows,
@@ -590,7 +590,7 @@ int kh_pages_copy(void* pages, int64_t planes, int64_t num_pages, int64_t page_b
  * then the lower beam; inside a beam the larger logit, then the lower token): out_scores (fp32),
  * out_tokens, out_parents (the beam, int32) and out_finished (given with finished: the parent's flag, or the
  * token is eos), each [groups, k].  k <= 64, beams <= 64, k <= beams * vocab (with finished: k <= beams).
- * Candidates are compared in float64.  Extends sample() (reference:
+ * Candidates are compared in float64.  No result shares memory with an input.  Extends sample() (reference:
  * packages/model-utils/src/sampling/index.ts:103-243) to several hypotheses. */
 int kh_beam_select(const void* logits, const int64_t* strides, const float* scores, const int32_t* finished, int64_t groups,
                    int64_t beams, int64_t vocab, int k, int64_t eos, float* out_scores, int32_t* out_tokens,

@@ -5,7 +5,7 @@
 // A finished beam has one continuation: itself, with the end token.  NaN, as a logit or a score, counts
 // as -inf.  Order: the larger score, then the lower beam, then the lower token.  Inside a beam the logits
 // decide, so only the k largest of each beam are scored, in float64.
-#include "common.h"
+#include "paged.h"
 
 using namespace kh;
 
@@ -191,7 +191,8 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
   if (lane == 0) part[w] = make_float2(m, s);
   // the wave's k best as order keys, in order
   uint64_t* out = best + w * k;
-  const float floor = order_value(kth_lane(order_bits(mine), k));
+  // (-inf at least: what kth_lane leaves may lie below it, where the bits are a NaN's)
+  const float floor = order_value(max(kth_lane(order_bits(mine), k), order_bits(-INFINITY)));
   int count = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -351,6 +352,10 @@ int kh_beam_select(const void* logits, const int64_t* strides, const float* scor
   if (groups == 0) return KH_OK;
   KH_REQUIRE(logits && strides && scores && out_scores && out_tokens && out_parents, "kh_beam_select: null pointer");
   const int64_t rows = groups * beams;
+  KH_REQUIRE(!overlap({ints(out_scores, groups * k), ints(out_tokens, groups * k), ints(out_parents, groups * k),
+                       ints(out_finished, groups * k)},
+                      {ints(scores, rows), ints(finished, rows)}),
+             "kh_beam_select: the results must not share memory with the inputs or each other");
   const int shift = (dtype == KH_BF16 ? 8 : 4) - 1;  // a row may start this far inside a 16-byte block
   const int runs = (int)((vocab + shift + kRun - 1) / kRun);
   const size_t sum_bytes = ((size_t)rows * runs * sizeof(float2) + 255) / 256 * 256;

@@ -358,12 +358,6 @@ bool rows_ok(int64_t rows, int64_t width, int64_t stride, int64_t num_pages) {
          num_pages <= INT32_MAX;
 }
 
-// Whether an output of n int32 values starting at `out` shares memory with an input of m at `in`.
-bool shares(const void* out, int64_t n, const void* in, int64_t m) {
-  const uintptr_t a = (uintptr_t)out, b = (uintptr_t)in;
-  return n > 0 && m > 0 && a < b + 4 * (uint64_t)m && b < a + 4 * (uint64_t)n;
-}
-
 unsigned blocks_for(int64_t n) {
   const int64_t b = (n + 255) / 256, most = 8 * (int64_t)cu_count();
   return (unsigned)(b < 1 ? 1 : (b < most ? b : most));
@@ -407,10 +401,10 @@ int kh_pages_fork(const int32_t* page_table, int64_t table_stride, const int32_t
   KH_REQUIRE((rows == 0 || (kv_lens && parents && new_lens)) && (rows == 0 || table_width == 0 || (page_table && new_table)) &&
                  (num_pages == 0 || (page_refs && new_refs)),
              "kh_pages_fork: null pointer");
-  const int64_t span = rows == 0 || table_width == 0 ? 0 : (rows - 1) * table_stride + table_width;
-  KH_REQUIRE(!shares(new_table, rows * table_width, page_table, span) && !shares(new_lens, rows, kv_lens, rows) &&
-                 !shares(new_refs, num_pages, page_refs, num_pages),
-             "kh_pages_fork: the results must not share memory with the inputs");
+  KH_REQUIRE(!overlap({ints(new_table, rows * table_width), ints(new_lens, rows), ints(new_refs, num_pages)},
+                      {table_span(page_table, table_stride, rows, table_width), ints(kv_lens, rows), ints(page_refs, num_pages),
+                       ints(parents, rows)}),
+             "kh_pages_fork: the results must not share memory with the inputs or each other");
   if (rows == 0 && num_pages == 0) return KH_OK;
   if (num_pages <= kForkPages && rows <= kForkRows && rows * table_width <= kForkEntries) {
     pages_fork_small_kernel<<<1, 1024, 0, stream()>>>(page_table, table_stride, kv_lens, page_refs, parents, (int)rows,
@@ -439,10 +433,16 @@ int kh_pages_reserve(int32_t* page_table, int64_t table_stride, int32_t* kv_lens
   KH_REQUIRE(rows <= kMaxRows, "kh_pages_reserve: %lld rows, at most %d", (long long)rows, kMaxRows);
   KH_REQUIRE(page_size >= 16 && page_size <= 4096 && (page_size & (page_size - 1)) == 0,
              "kh_pages_reserve: page size %lld is not a power of two from 16 to 4096", (long long)page_size);
-  KH_REQUIRE(table_width * page_size <= (1 << 30), "kh_pages_reserve: the page table passes 2^30 rows");
+  // (the pages that a call may need are counted in 32 bits)
+  KH_REQUIRE(table_width <= (1 << 30) && table_width * page_size <= (1 << 30) && rows * table_width <= INT32_MAX,
+             "kh_pages_reserve: the page table passes 2^30 rows, or 2^31 entries");
   KH_REQUIRE(info && (rows == 0 || (kv_lens && counts && moves)) && (rows == 0 || table_width == 0 || page_table) &&
                  (num_pages == 0 || page_refs),
              "kh_pages_reserve: null pointer");
+  KH_REQUIRE(!overlap({table_span(page_table, table_stride, rows, table_width), ints(kv_lens, rows), ints(page_refs, num_pages),
+                       ints(moves, 2 * rows), ints(info, 3)},
+                      {ints(counts, rows)}),
+             "kh_pages_reserve: the operands must not share memory with each other");
   pages_reserve_kernel<<<1, kOne, 0, stream()>>>(page_table, table_stride, kv_lens, page_refs, counts, (int)rows,
                                                  (int)table_width, (int)num_pages, log2_of(page_size), moves, info);
   KH_CHECK_LAUNCH();
@@ -459,9 +459,9 @@ int kh_pages_compact(const int32_t* page_table, int64_t table_stride, const int3
   KH_REQUIRE(info && (max_moves == 0 || moves) && (num_pages == 0 || (page_refs && new_refs)) &&
                  (rows == 0 || table_width == 0 || (page_table && new_table)),
              "kh_pages_compact: null pointer");
-  const int64_t span = rows == 0 || table_width == 0 ? 0 : (rows - 1) * table_stride + table_width;
-  KH_REQUIRE(!shares(new_table, rows * table_width, page_table, span) && !shares(new_refs, num_pages, page_refs, num_pages),
-             "kh_pages_compact: the results must not share memory with the inputs");
+  KH_REQUIRE(!overlap({ints(new_table, rows * table_width), ints(new_refs, num_pages), ints(moves, 2 * max_moves), ints(info, 2)},
+                      {table_span(page_table, table_stride, rows, table_width), ints(page_refs, num_pages)}),
+             "kh_pages_compact: the results must not share memory with the inputs or each other");
   int32_t* to = nullptr;
   if (num_pages > 0) {
     to = (int32_t*)scratch_alloc((size_t)num_pages * 4);

@@ -150,7 +150,8 @@ def pages_reserve(page_table: Tensor, kv_lens: Tensor, page_refs: Tensor, counts
     too, is replaced; its contents have to follow: pages_copy(pages, moves, info).
 
     Returns (moves int32 [rows, 2], info int32 [3]): pairs (from, to), and their number, the pages that were
-    missing and the rows that the table is too narrow for.  If any were, nothing has changed."""
+    missing and the rows that the table is too narrow for.  If any were, nothing has changed.  No two of the tensors
+    share memory."""
     if out is None:
         rows = page_table.shape[0]
         out = (_wrap(_new(page_table, (rows, 2))), _wrap(_new(page_table, (3,))))
@@ -188,7 +189,8 @@ def beam_select(logits: Tensor, scores: Tensor, k: Optional[int] = None, finishe
     eos_token_id, at their score.
 
     Returns (scores, tokens, parents, finished), each [groups, k] and best first: log_softmax(logits)[token] +
-    scores[parent], ties to the lower beam and token; finished is None without flags given."""
+    scores[parent], ties to the lower beam and token; finished is None without flags given.  out: the four results,
+    which share no memory with the inputs."""
     groups, beams = logits.shape[0], logits.shape[1]
     k = beams if k is None else int(k)
     if out is None:

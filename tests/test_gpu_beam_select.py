@@ -53,6 +53,15 @@ def test_best_continuations(hip, dtype, groups, beams, vocab, k):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("vocab", [33, 100, 2060, 8200])
+@pytest.mark.parametrize("k", [63, 64])
+def test_as_many_as_lanes(hip, dtype, vocab, k):
+    """k at and below the 64 lanes of a wave, the last wave's being mostly behind the row's end."""
+    x, xh = logits_of(vocab + k, (1, 2, vocab), dtype)
+    check(x, xh, np.array([[-1.5, -1.0]]), k)
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 def test_finished_beams_go_on_as_themselves(hip, dtype):
     x, xh = logits_of(3, (4, 5, 2000), dtype)
     s = -5 * np.random.default_rng(4).random((4, 5))
@@ -151,3 +160,15 @@ def test_refusals(hip):
             F.beam_select(x, s, 2, f, eos)
     with pytest.raises(KandleHipError, match="beams"):
         F.beam_select(F.zeros((1, 65, 10)), F.zeros((1, 65)), 2)
+
+
+def test_results_in_place_of_inputs_are_refused(hip):
+    x, s, f = F.zeros((1, 2, 10)), F.zeros((1, 2)), F.zeros((1, 2), "int32")
+    new = lambda: F.zeros((1, 2), "int32")  # noqa: E731
+    with pytest.raises(KandleHipError, match="share memory"):
+        F.beam_select(x, s, 2, out=(s, new(), new(), None))
+    with pytest.raises(KandleHipError, match="share memory"):
+        F.beam_select(x, s, 2, f, 1, out=(F.zeros((1, 2)), new(), new(), f))
+    same = new()
+    with pytest.raises(KandleHipError, match="share memory"):
+        F.beam_select(x, s, 2, out=(F.zeros((1, 2)), same, same, None))

@@ -5,6 +5,7 @@ import pytest
 from helpers import seeded
 from kandle_amd import Tensor
 from kandle_amd import functional as F
+from kandle_amd import _lib
 from kandle_amd._lib import KandleHipError
 from kandle_amd.graphs import HipGraph
 from oracle import paged as op
@@ -166,3 +167,26 @@ def test_refusals(hip):
         F.pages_reserve(i32(np.zeros((2049, 1))), i32(np.zeros(2049)), f, i32(np.zeros(2049)), 16)
     with pytest.raises(KandleHipError, match="multiple of 16"):
         F.pages_copy(F.zeros((4, 1, 1, 3)), i32([[0, 1]]), i32([1]))
+
+
+def test_operands_that_share_memory_are_refused(hip):
+    new = lambda *s: i32(np.zeros(s))  # noqa: E731
+    t, n, f, p = new(2, 3), new(2), new(5), new(2)
+    for lens in (n, p):
+        with pytest.raises(KandleHipError, match="share memory"):
+            F.pages_fork(t, n, f, p, out=(new(2, 3), lens, new(5)))
+    with pytest.raises(KandleHipError, match="share memory"):
+        F.pages_reserve(t, n, f, n, 16)
+    both = new(7)
+    with pytest.raises(KandleHipError, match="share memory"):
+        F.pages_reserve(t, n, f, p, 16, out=(F.view(F.narrow(both, 0, 0, 4), (2, 2)), F.narrow(both, 0, 3, 3)))
+    F.pages_reserve(t, n, f, p, 16, out=(F.view(F.narrow(both, 0, 0, 4), (2, 2)), F.narrow(both, 0, 4, 3)))
+    with pytest.raises(KandleHipError, match="share memory"):
+        F.pages_compact(t, f, out=(new(2, 3), f, new(2, 2), new(2)))
+
+
+def test_tables_past_the_counters_are_refused(hip):
+    a = i32(np.zeros(64))
+    with pytest.raises(KandleHipError, match="2\\^31 entries"):   # refused on the host, whatever the pointers are
+        _lib.call("kh_pages_reserve", a.handle.data_ptr(), 1 << 26, a.handle.data_ptr(), a.handle.data_ptr(), a.handle.data_ptr(), 64,
+                  1 << 26, 64, 16, a.handle.data_ptr(), a.handle.data_ptr())
