@@ -25,6 +25,8 @@ class PagedKVCache:
                  max_seq_len: int, page_size: int = 16, dtype: str = "bfloat16"):
         if num_pages < 1 or max_sequences < 1 or max_seq_len < 1:
             raise ValueError(f"PagedKVCache: {num_pages} pages, {max_sequences} sequences of {max_seq_len} rows")
+        if max_sequences > 2048 or max_seq_len > 1 << 30:
+            raise ValueError(f"PagedKVCache: {max_sequences} sequences of {max_seq_len} rows, at most 2048 of 2^30")
         if page_size < 16 or page_size > 4096 or page_size & (page_size - 1):
             raise ValueError(f"PagedKVCache: page size {page_size} is not a power of two from 16 to 4096")
         self.num_layers, self.page_size, self.num_pages = num_layers, page_size, num_pages

@@ -431,6 +431,8 @@ class Qwen3ForCausalLM:
                         page_size: int = 16) -> PagedKVCache:
         """A paged cache for this model's layers, in its activation dtype."""
         c = self.cfg
+        if c.head_dim not in (64, 128):
+            raise ValueError(f"new_paged_cache: paged attention takes heads of 64 or 128 values, not {c.head_dim}")
         return PagedKVCache(c.num_hidden_layers, c.num_key_value_heads, c.head_dim, num_pages, max_sequences,
                             self.max_seq_len if max_seq_len is None else max_seq_len, page_size, self.act)
 

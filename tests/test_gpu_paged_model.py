@@ -160,3 +160,12 @@ def test_beam_refusals(hip):
     with pytest.raises(RuntimeError, match="pages are missing"):
         model.generate_beams([[1, 2, 3]], 4, 40, num_pages=4)
     model.dispose()
+
+
+def test_heads_that_paged_attention_does_not_take_are_refused(hip):
+    cfg, model, _ = make(head_dim=32)
+    with pytest.raises(ValueError, match="64 or 128"):
+        model.new_paged_cache(2, 8)
+    with pytest.raises(ValueError, match="64 or 128"):
+        model.generate_beams([[1, 2]], 2, 4)
+    model.dispose()

@@ -158,3 +158,10 @@ def test_beam_select_refuses():
             kernels.beam_select(*good[:i], bad, *good[i + 1:])
     with pytest.raises(ValueError, match="eos_token_id"):
         kernels.beam_select(x, s, f, 3, None, s, f, f, f)
+
+
+def test_caches_past_the_kernels_limits_are_refused():
+    from kandle_amd.model_utils import PagedKVCache
+    for sequences, rows in ((2049, 64), (2, (1 << 30) + 1)):
+        with pytest.raises(ValueError, match="at most 2048 of 2\\^30"):
+            PagedKVCache(2, 2, 64, 4, sequences, rows)
