@@ -175,24 +175,28 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
   }
   // id of value i; values behind the row's end are -inf like some inside it, and told apart by it
   auto id_of = [&](int i) { return start + (i / E) * 64 * E + i % E; };
-  float mine = -INFINITY;
+  float mine = -INFINITY;  // (a maximum passes over NaN)
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    v[i] = no_nan(v[i]);
-    mine = fmaxf(mine, v[i]);
-  }
+  for (int i = 0; i < kPer; ++i) mine = __builtin_fmaxf(mine, v[i]);
   const float m = wave_max_dpp(mine);
-  float s = 0.f;
-  if (m > -INFINITY) {
+  // (-inf at least: what kth_lane leaves may lie below it, where the bits are a NaN's)
+  const float floor = order_value(max(kth_lane(order_bits(mine), k), order_bits(-INFINITY)));
+  auto sum = [&] {
+    float s = 0.f;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) s += fast_exp2((v[i] - m) * kLog2e);
-    s = wave_sum(s);
+    return wave_sum(s);
+  };
+  float s = m > -INFINITY ? sum() : 0.f;
+  // NaN counts as -inf, which matters where the sum has found one or -inf is among the k largest
+  if (s != s || floor == -INFINITY) {
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) v[i] = no_nan(v[i]);
+    s = m > -INFINITY ? sum() : 0.f;
   }
   if (lane == 0) part[w] = make_float2(m, s);
   // the wave's k best as order keys, in order
   uint64_t* out = best + w * k;
-  // (-inf at least: what kth_lane leaves may lie below it, where the bits are a NaN's)
-  const float floor = order_value(max(kth_lane(order_bits(mine), k), order_bits(-INFINITY)));
   int count = 0;
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
@@ -212,6 +216,7 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
     for (int j = lane; j < count; j += 64) {
       const uint64_t key = room[w][j];
       int rank = 0;
+#pragma unroll 8
       for (int i = 0; i < count; ++i) rank += room[w][i] > key;
       if (rank < k) out[rank] = key;
     }
@@ -245,6 +250,7 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
   for (int j = threadIdx.x; j < kRunWaves * k; j += kRunWaves * 64) {
     const uint64_t key = best[j];
     int rank = 0;
+#pragma unroll 8
     for (int i = 0; i < kRunWaves * k; ++i) rank += best[i] > key || (best[i] == key && i < j);
     if (rank < k) keys[o * k + rank] = key;
   }
