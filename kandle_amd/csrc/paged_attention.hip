@@ -10,6 +10,8 @@
 // Work is split over tiles of packed rows and over chunks of `chunk` keys; where a tile's keys make more
 // than one chunk, each chunk leaves (O, m, l) partials and paged_merge_kernel joins them in chunk order, so
 // a result does not depend on timing.
+#include <cmath>
+
 #include "paged_rows.h"
 
 using namespace kh;
@@ -134,16 +136,20 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_row_kernel(const
 // A part of a launch of `tiles` tiles per kv head, of which `there` hold rows as far as can be told here: its keys in as
 // many equal chunks (multiples of 128 keys, `least` at least) as make no more than `most` workgroups with keys, and
 // partials (one per row and chunk) of no more than most_parts rows.  With f the part of the keys that the tiles do not
-// see on average, n chunks leave there (n (1 - f) + f) workgroups with keys.
-PagedPart part_of(const PagedCall& c, int64_t tiles, int64_t there, int least, int64_t most, int64_t most_parts) {
+// see on average, n chunks leave there (n (1 - f) + f) workgroups with keys.  Where that gives one chunk and a part of
+// another (`uneven`), a second, shorter one shares the places that one each would leave empty: 3000 tokens of 9000 keys
+// 269 -> 228 us, six chunks of up to 300 of 2600 96 -> 85; beside many workgroups of the other kind it loses (three
+// of up to 300 and 20 tokens 63 -> 76), and so do a third and later chunk like it.
+PagedPart part_of(const PagedCall& c, int64_t tiles, int64_t there, int least, int64_t most, int64_t most_parts, bool uneven) {
   const int64_t len = c.pb.max_len, rows = (int64_t)c.pb.tokens * c.hq;
   if (there < 1) there = 1;
   if (len <= least) return PagedPart{(int)(tiles * c.hkv), least, 1};
   const double f = c.causal ? 0.5 * (c.max_new < len ? c.max_new : len) / len : 0.0;
-  int64_t n = (int64_t)(((double)most / ((double)there * c.hkv) - f) / (1.0 - f));
-  if (n > most_parts / rows) n = most_parts / rows;
-  if (n < 1) n = 1;
-  int64_t chunk = ((len + n - 1) / n + 127) / 128 * 128;
+  double n = ((double)most / ((double)there * c.hkv) - f) / (1.0 - f);
+  if (!uneven || n < 1.1 || n >= 2.0) n = (double)(int64_t)n;
+  if (n > (double)(most_parts / rows)) n = (double)(most_parts / rows);
+  if (n < 1.0) n = 1.0;
+  int64_t chunk = ((int64_t)std::ceil(len / n) + 127) / 128 * 128;
   if (chunk < least) chunk = least;
   return PagedPart{(int)(tiles * c.hkv), (int)chunk, (int)((len + chunk - 1) / chunk)};
 }
@@ -190,9 +196,11 @@ int launch(const PagedCall& c) {
   // with a quarter or a half more of them 86.3, with twice as many 88.1, with chunk lengths of powers of two 82.9.
   // 512 keys of a tile at least: partials cost more than shorter chunks gain.  Beside a prompt's many rows, whose
   // workgroups take as long, few rows need no short chunks: partials of 2^18 rows at most.
-  const PagedPart few =
-      part_of(c, few_tiles, few_there, 128, cus * (sizeof(T) == 4 && D == 128 ? 1 : 2), many_too ? 1 << 18 : INT64_MAX);
-  const PagedPart many = part_of(c, many_tiles, many_tiles, 512, cus * (waves == 8 ? 1 : 2), INT64_MAX);
+  const int64_t places = cus * (waves == 8 ? 1 : 2);
+  const PagedPart few = part_of(c, few_tiles, few_there, 128, cus * (sizeof(T) == 4 && D == 128 ? 1 : 2),
+                                many_too ? 1 << 18 : INT64_MAX, !many_too);
+  const PagedPart many =
+      part_of(c, many_tiles, many_tiles, 512, places, INT64_MAX, !few_too || few_there * c.hkv < places / 2);
   const int few_chunks = few_too ? few.used : 1, many_chunks = many_too ? many.used : 1;
   const int chunks = few_chunks > many_chunks ? few_chunks : many_chunks;
   KH_REQUIRE(chunks <= 65535 && (int64_t)few.columns * few_chunks + (int64_t)many.columns * many_chunks <= INT32_MAX,
