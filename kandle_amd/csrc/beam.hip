@@ -135,6 +135,10 @@ __device__ __forceinline__ void wave_best(Cand (&c)[N], int k, Cand* room, Cand*
 // A workgroup takes a run of 8192 logits of one row, 32 per lane in registers: their maximum, the sum of
 // exponentials relative to it, and the k largest in order.  Rows may start anywhere: the lanes' 16-byte loads
 // lie on the 16-byte grid of the memory, and those that cross a row's ends are made value by value.
+//
+// Bound by the vector ALU (13.5 instructions per logit, four of them the exponential's) and the selection's chain: 128
+// rows of 151936 bf16 logits, of which a quarter have finished, 16 us (29 MB); four fp32 rows 7.7.  Runs of twice the
+// length in as many registers are slower (22.4 -> 25.3 us a call): fewer waves hide the chain.
 constexpr int kPer = 32, kRunWaves = 4, kRun = kPer * 64 * kRunWaves;
 template <typename T>
 __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __restrict__ logits, int64_t sg, int64_t sb,
@@ -256,7 +260,8 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
   }
 }
 
-// A workgroup per group: the sums of its beams, then the k best of the runs' candidates, scored in float64.
+// A workgroup per group: the sums of its beams, then the k best of the runs' candidates, scored in float64.  Latency:
+// 5.3 us for one group of four beams, 8 for sixteen groups of eight (1216 candidates each).
 constexpr int kMergeWaves = 16, kSlots = 2;
 __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
     const float2* __restrict__ sums, const uint64_t* __restrict__ keys, const float* __restrict__ scores,

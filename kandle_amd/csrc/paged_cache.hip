@@ -4,7 +4,7 @@
 // The bookkeeping stays on the device, so that a captured step replays it: a page is free while its
 // reference count is 0, and new pages are the lowest free ones in row order, which makes every result a
 // function of the arguments alone (the counts are changed by integer atomics, whose order does not
-// matter).
+// matter).  These kernels are short: each is bound by its chain of dependent loads and scans.
 #include "paged.h"
 
 using namespace kh;
@@ -16,7 +16,8 @@ struct WriteStrides {
   int64_t kt, kh, vt, vh, kp, kph, kpr, vp, vph, vpr;
 };
 
-// A workgroup takes one token: its threads copy the heads' K and V rows in pieces of E.
+// A workgroup takes one token: its threads copy the heads' K and V rows in pieces of E.  6600 bf16 tokens of 8 heads
+// of 128: 11 us, 4.9 TB/s read and written, what a large copy reaches; one token of eight sequences: 2.8 us.
 template <typename E>
 __global__ __launch_bounds__(256) void paged_write_kernel(const E* __restrict__ K, const E* __restrict__ V,
                                                           E* __restrict__ KP, E* __restrict__ VP, PagedBatch pb, int hkv,
@@ -138,7 +139,8 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int* total) {
 // its last page.  The page of a partly filled tail is kept if no other row holds it, or if all its holders
 // grow and this is the last of them; otherwise the row gets a copy of it, also a new page.  (One row after
 // the other, each copying while the count is above 1, gives the same.)  Nothing changes unless all rows
-// can grow.
+// can grow.  64 rows, 64 sharing tails, in a pool of 685 pages: 7.8 us (two scans of the counts to the last page
+// needed, 1024 at a time).
 __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict__ table, int64_t stride,
                                                              int32_t* __restrict__ lens, int32_t* __restrict__ refs,
                                                              const int32_t* __restrict__ counts, int rows, int width,
@@ -266,7 +268,7 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
 
 // ---- compact ----------------------------------------------------------------------------------
 // One workgroup: with n live pages, the i-th live page at or behind n moves to the i-th free page before n.
-// to[page]: where a page is afterwards.
+// to[page]: where a page is afterwards.  4000 pages: 11 us (two scans), and 4.7 for the table.
 __global__ __launch_bounds__(kOne) void pages_compact_kernel(const int32_t* __restrict__ refs, int num_pages,
                                                              int32_t* __restrict__ new_refs, int32_t* __restrict__ to,
                                                              int32_t* __restrict__ moves, int max_moves,
@@ -320,7 +322,8 @@ __global__ __launch_bounds__(256) void pages_rename_kernel(const int32_t* __rest
 }
 
 // ---- copy -------------------------------------------------------------------------------------
-// A workgroup copies pieces of 16 KiB: piece i of move m of plane l, in the order (move, plane, piece).
+// A workgroup copies pieces of 16 KiB: piece i of move m of plane l, in the order (move, plane, piece).  494 MB read and
+// written in 103 us, 4.8 TB/s, what a large copy reaches; a beam step's 23 MB in 5.6.
 constexpr int kPiece = 16384;
 __global__ __launch_bounds__(256) void pages_copy_kernel(uint8_t* __restrict__ pages, int64_t planes, int64_t plane_bytes,
                                                          int64_t page_bytes, int num_pages,

@@ -1,7 +1,7 @@
 """beam_select against the sort of all continuations in float64 (oracle/paged.py).
 
 Tokens, parents and flags are exact.  Scores: log sum exp from fp32 exponentials of arguments x - max (the rounding
-of the argument, |x - max| u, weighs with the term's share; here |x - max| < 64) and fp32 sums of 1024, in all below
+of the argument, |x - max| u, weighs with the term's share; here |x - max| < 64) and fp32 sums of 8192 (42 additions on the way of a term), in all below
 80 u absolute, and one rounding of the result: 2^-24 |score|.  u = 2^-24."""
 import numpy as np
 import pytest
