@@ -136,11 +136,11 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int* total) {
 }
 
 // One workgroup.  A row that grows from len to len + count takes a new page for every table entry behind
-// its last page.  The page of a partly filled tail is kept if no other row holds it, or if all its holders
-// grow and this is the last of them; otherwise the row gets a copy of it, also a new page.  (One row after
-// the other, each copying while the count is above 1, gives the same.)  Nothing changes unless all rows
-// can grow.  64 rows, 64 sharing tails, in a pool of 685 pages: 7.8 us (two scans of the counts to the last page
-// needed, 1024 at a time).
+// its last page.  Of the rows that grow on one partly filled page, each gets a copy of it, also a new page, as long as
+// another row holds it, too: row after row, while the count less the copies before is above 1.  Nothing changes
+// unless all rows can grow.  64 rows, 64 sharing tails, in a pool of 685 pages: 5.9 us, a chain of four loads and three scans; the
+// free pages among the first kKept * 1024 keep their places from the count, which has to come first, to the writes.
+constexpr int kKept = 4;
 __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict__ table, int64_t stride,
                                                              int32_t* __restrict__ lens, int32_t* __restrict__ refs,
                                                              const int32_t* __restrict__ counts, int rows, int width,
@@ -151,22 +151,35 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
   __shared__ int before[kMaxRows];  // new pages of the rows before this one
   __shared__ int number[kMaxRows];  // copies of the rows before this one
   __shared__ int waves[kOne / 64];
+  __shared__ int2 flags[kOne / 64];
+  constexpr int PER = kMaxRows / kOne;
   const int64_t page = int64_t(1) << page_log;
-  int bad = 0;
-  for (int s = threadIdx.x; s < rows; s += kOne) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  int held[PER], grows[PER];  // this thread's rows: holders of the tail page, new rows
+  bool bad[PER];
+#pragma unroll
+  for (int i = 0; i < PER; ++i) {
+    const int s = i * kOne + threadIdx.x;
+    held[i] = 0;
+    grows[i] = 0;
+    bad[i] = false;
+    if (s >= rows) continue;
     const int64_t len = max(lens[s], 0), end = len + max(counts[s], 0);
     int t = -1, f = -1;  // -1: the row does not grow
     if (end > len && end > width * page) {
-      ++bad;
+      bad[i] = true;
     } else if (end > len) {
       f = (int)((len + page - 1) >> page_log);
+      grows[i] = (int)((end + page - 1) >> page_log) - f;
       if (len & (page - 1)) {
         t = table[s * stride + (len >> page_log)];
         if ((unsigned)t >= (unsigned)num_pages) {
           t = -1;
           --f;  // no page in the tail's place: a new one, with nothing to copy
-        } else if (refs[t] <= 1) {
-          t = -1;
+          ++grows[i];
+        } else {
+          held[i] = refs[t];
+          if (held[i] <= 1) t = -1;
         }
       }
     }
@@ -176,39 +189,42 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
   }
   __syncthreads();
   int needed = 0, copied = 0, too_long = 0;
-  int mine[kMaxRows / kOne];  // whether this thread's rows copy their tail
-  for (int i = 0; i < kMaxRows / kOne; ++i) mine[i] = 0;
+  bool mine[PER];  // whether this thread's rows copy their tail
 #pragma unroll
-  for (int i = 0; i < kMaxRows / kOne; ++i) {
-    const int s = i * kOne + threadIdx.x;
+  for (int i = 0; i < PER; ++i) {
+    mine[i] = false;
     if (i * kOne >= rows) break;
-    int need = 0;
-    if (s < rows && first[s] >= 0) {
-      const int t = tail[s];
-      if (t >= 0) {
-        int sharers = 0, last = 0;
-        for (int r = 0; r < rows; ++r)
-          if (tail[r] == t) {
-            ++sharers;
-            last = r;
-          }
-        mine[i] = !(last == s && refs[t] <= sharers);
-      }
-      need = (int)(((int64_t)max(lens[s], 0) + counts[s] + page - 1) >> page_log) - first[s] + mine[i];
+    const int s = i * kOne + threadIdx.x;
+    const int t = s < rows ? tail[s] : -1;
+    if (t >= 0) {
+      int sharers = 0;  // before this row
+#pragma unroll 8
+      for (int r = 0; r < s; ++r) sharers += tail[r] == t;
+      mine[i] = held[i] - sharers > 1;
     }
-    int total = 0, moved = 0;
-    const int b = block_scan(need, waves, &total), m = block_scan(mine[i], waves, &moved);
+    // prefix sums of the new pages and of the copies
+    const uint64_t copy = __ballot(mine[i]), wrong = __ballot(bad[i]);
+    if (lane == 0) flags[w] = make_int2(__popcll(copy), __popcll(wrong));
+    int total = 0;
+    const int b = block_scan(grows[i] + mine[i], waves, &total);
+    int m = __popcll(copy & ((1ull << lane) - 1)), moved = 0;
+#pragma unroll
+    for (int k = 0; k < kOne / 64; ++k) {
+      if (k < w) m += flags[k].x;
+      moved += flags[k].x;
+      too_long += flags[k].y;
+    }
     if (s < rows) {
       before[s] = needed + b;
       number[s] = copied + m;
     }
     needed += total;
     copied += moved;
+    if (PER > 1) __syncthreads();  // (the flags are read)
   }
-  block_scan(bad, waves, &too_long);
   __syncthreads();  // every row has read the others' tails
 #pragma unroll
-  for (int i = 0; i < kMaxRows / kOne; ++i) {
+  for (int i = 0; i < PER; ++i) {
     const int s = i * kOne + threadIdx.x;
     if (s < rows) {
       if (mine[i])
@@ -217,9 +233,39 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
         tail[s] = -1;
     }
   }
-  // the free pages, counted up to the number needed
-  int found = 0;
-  for (int64_t p0 = 0; p0 < num_pages && found < needed; p0 += kOne) {
+  // the r-th lowest free page goes to the row whose new pages r lies among
+  auto give = [&](int p, int r) {
+    int lo = 0, hi = rows;  // the last row with before[row] <= r (rows without new pages share the next one's)
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if (before[mid] <= r)
+        lo = mid;
+      else
+        hi = mid;
+    }
+    const int at = r - before[lo];
+    table[lo * stride + first[lo] + at] = p;
+    refs[p] = 1;
+    if (at == 0 && tail[lo] >= 0) {
+      moves[2 * number[lo]] = tail[lo];
+      moves[2 * number[lo] + 1] = p;
+    }
+  };
+  // the free pages, counted up to the number needed; place[i]: this thread's i-th page among them
+  int found = 0, kept = 0, place[kKept];
+#pragma unroll
+  for (int i = 0; i < kKept; ++i) {
+    place[i] = -1;
+    const int64_t p0 = (int64_t)i * kOne, p = p0 + threadIdx.x;
+    if (p0 >= num_pages || found >= needed) continue;  // (the same for every thread)
+    const bool free = p < num_pages && refs[p] <= 0;
+    int n = 0;
+    const int r = found + block_scan(free, waves, &n);
+    if (free && r < needed) place[i] = r;
+    found += n;
+  }
+  kept = found;
+  for (int64_t p0 = (int64_t)kKept * kOne; p0 < num_pages && found < needed; p0 += kOne) {
     const int64_t p = p0 + threadIdx.x;
     int n = 0;
     block_scan(p < num_pages && refs[p] <= 0, waves, &n);
@@ -233,31 +279,17 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
   }
   if (!ok) return;
   __syncthreads();
-  // the r-th lowest free page goes to the row whose new pages r lies among
-  found = 0;
-  for (int64_t p0 = 0; p0 < num_pages && found < needed; p0 += kOne) {
+#pragma unroll
+  for (int i = 0; i < kKept; ++i)
+    if (place[i] >= 0) give(i * kOne + threadIdx.x, place[i]);
+  found = kept;
+  for (int64_t p0 = (int64_t)kKept * kOne; p0 < num_pages && found < needed; p0 += kOne) {
     const int64_t p = p0 + threadIdx.x;
     const bool free = p < num_pages && refs[p] <= 0;
     int n = 0;
     const int r = found + block_scan(free, waves, &n);
     found += n;
-    if (free && r < needed) {
-      int lo = 0, hi = rows;  // the last row with before[row] <= r (rows without new pages share the next one's)
-      while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (before[mid] <= r)
-          lo = mid;
-        else
-          hi = mid;
-      }
-      const int at = r - before[lo];
-      table[lo * stride + first[lo] + at] = (int)p;
-      refs[p] = 1;
-      if (at == 0 && tail[lo] >= 0) {
-        moves[2 * number[lo]] = tail[lo];
-        moves[2 * number[lo] + 1] = (int)p;
-      }
-    }
+    if (free && r < needed) give((int)p, r);
   }
   __syncthreads();
   for (int s = threadIdx.x; s < rows; s += kOne) {

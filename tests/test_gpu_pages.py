@@ -50,6 +50,22 @@ def test_fork_and_reserve(hip, rows, width, pages, page):
         table, lens, refs = after[:3]
 
 
+@pytest.mark.parametrize("rows,free,count", [(40, 0.02, 100), (40, 0.02, 33), (1100, 0.6, 80), (2048, 0.9, 60), (2048, 0.3, 40), (7, 0.0, 1)])
+def test_reserve_from_a_large_pool(hip, rows, free, count):
+    """Free pages few and far between, or behind the first thousands; enough of them or not; rows that are too long."""
+    r = np.random.default_rng(rows + count)
+    pages, width, page = 11000, 8, 16
+    refs = (r.random(pages) >= free).astype(np.int64)
+    lens = r.integers(0, 60, rows)
+    table = np.where(np.arange(width) < -(-lens // page)[:, None], r.integers(0, pages, (rows, width)), -1)
+    refs[table[table >= 0]] += 1                     # some are shared
+    for counts in (r.integers(-1, count, rows), np.full(rows, 1), np.where(np.arange(rows) == rows - 1, 1000, 1)):
+        want = op.pages_reserve(table, lens, refs, counts, page)
+        t, n, f = i32(table), i32(lens), i32(refs)
+        moves, info = F.pages_reserve(t, n, f, i32(counts), page)
+        same([t, n, f, moves, info], want)
+
+
 def test_the_last_sharer_keeps_the_tail_page(hip):
     table = np.array([[3, 1, -1], [3, 1, -1], [3, 1, -1], [5, 2, -1], [5, 2, -1]])
     lens, refs = np.array([20, 20, 20, 31, 31]), np.array([0, 3, 2, 3, 0, 2, 0, 0])
