@@ -135,10 +135,32 @@ __device__ __forceinline__ int block_scan(int v, int* waves, int* total) {
   return before + inc - v;
 }
 
+// The same for two flags at once: the number of threads before this one that have them.
+__device__ __forceinline__ int2 block_places(bool a, bool b, int2* waves, int2* total) {
+  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+  const uint64_t ma = __ballot(a), mb = __ballot(b), below = (1ull << lane) - 1;
+  __syncthreads();  // the previous use of `waves` is over
+  if (lane == 0) waves[w] = make_int2(__popcll(ma), __popcll(mb));
+  __syncthreads();
+  int2 before = make_int2(__popcll(ma & below), __popcll(mb & below)), all = make_int2(0, 0);
+#pragma unroll
+  for (int i = 0; i < kOne / 64; ++i) {
+    const int2 n = waves[i];
+    if (i < w) {
+      before.x += n.x;
+      before.y += n.y;
+    }
+    all.x += n.x;
+    all.y += n.y;
+  }
+  *total = all;
+  return before;
+}
+
 // One workgroup.  A row that grows from len to len + count takes a new page for every table entry behind
 // its last page.  Of the rows that grow on one partly filled page, each gets a copy of it, also a new page, as long as
 // another row holds it, too: row after row, while the count less the copies before is above 1.  Nothing changes
-// unless all rows can grow.  64 rows, 64 sharing tails, in a pool of 685 pages: 5.9 us, a chain of four loads and three scans; the
+// unless all rows can grow.  64 rows, 64 sharing tails, in a pool of 685 pages: 6 us, a chain of four loads and three scans; the
 // free pages among the first kKept * 1024 keep their places from the count, which has to come first, to the writes.
 constexpr int kKept = 4;
 __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict__ table, int64_t stride,
@@ -154,7 +176,6 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
   __shared__ int2 flags[kOne / 64];
   constexpr int PER = kMaxRows / kOne;
   const int64_t page = int64_t(1) << page_log;
-  const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   int held[PER], grows[PER];  // this thread's rows: holders of the tail page, new rows
   bool bad[PER];
 #pragma unroll
@@ -202,25 +223,16 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
       for (int r = 0; r < s; ++r) sharers += tail[r] == t;
       mine[i] = held[i] - sharers > 1;
     }
-    // prefix sums of the new pages and of the copies
-    const uint64_t copy = __ballot(mine[i]), wrong = __ballot(bad[i]);
-    if (lane == 0) flags[w] = make_int2(__popcll(copy), __popcll(wrong));
     int total = 0;
-    const int b = block_scan(grows[i] + mine[i], waves, &total);
-    int m = __popcll(copy & ((1ull << lane) - 1)), moved = 0;
-#pragma unroll
-    for (int k = 0; k < kOne / 64; ++k) {
-      if (k < w) m += flags[k].x;
-      moved += flags[k].x;
-      too_long += flags[k].y;
-    }
+    int2 sums;
+    const int b = block_scan(grows[i] + mine[i], waves, &total), m = block_places(mine[i], bad[i], flags, &sums).x;
     if (s < rows) {
       before[s] = needed + b;
       number[s] = copied + m;
     }
     needed += total;
-    copied += moved;
-    if (PER > 1) __syncthreads();  // (the flags are read)
+    copied += sums.x;
+    too_long += sums.y;
   }
   __syncthreads();  // every row has read the others' tails
 #pragma unroll
@@ -259,17 +271,17 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
     const int64_t p0 = (int64_t)i * kOne, p = p0 + threadIdx.x;
     if (p0 >= num_pages || found >= needed) continue;  // (the same for every thread)
     const bool free = p < num_pages && refs[p] <= 0;
-    int n = 0;
-    const int r = found + block_scan(free, waves, &n);
+    int2 n;
+    const int r = found + block_places(free, false, flags, &n).x;
     if (free && r < needed) place[i] = r;
-    found += n;
+    found += n.x;
   }
   kept = found;
   for (int64_t p0 = (int64_t)kKept * kOne; p0 < num_pages && found < needed; p0 += kOne) {
     const int64_t p = p0 + threadIdx.x;
-    int n = 0;
-    block_scan(p < num_pages && refs[p] <= 0, waves, &n);
-    found += n;
+    int2 n;
+    block_places(p < num_pages && refs[p] <= 0, false, flags, &n);
+    found += n.x;
   }
   const bool ok = found >= needed && too_long == 0;
   if (threadIdx.x == 0) {
@@ -286,9 +298,9 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
   for (int64_t p0 = (int64_t)kKept * kOne; p0 < num_pages && found < needed; p0 += kOne) {
     const int64_t p = p0 + threadIdx.x;
     const bool free = p < num_pages && refs[p] <= 0;
-    int n = 0;
-    const int r = found + block_scan(free, waves, &n);
-    found += n;
+    int2 n;
+    const int r = found + block_places(free, false, flags, &n).x;
+    found += n.x;
     if (free && r < needed) give((int)p, r);
   }
   __syncthreads();
@@ -300,12 +312,13 @@ __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict
 
 // ---- compact ----------------------------------------------------------------------------------
 // One workgroup: with n live pages, the i-th live page at or behind n moves to the i-th free page before n.
-// to[page]: where a page is afterwards.  4000 pages: 11 us (two scans), and 4.7 for the table.
+// to[page]: where a page is afterwards.  4000 pages: 8.6 us (two scans), and 4.7 for the table.
 __global__ __launch_bounds__(kOne) void pages_compact_kernel(const int32_t* __restrict__ refs, int num_pages,
                                                              int32_t* __restrict__ new_refs, int32_t* __restrict__ to,
                                                              int32_t* __restrict__ moves, int max_moves,
                                                              int32_t* __restrict__ info) {
   __shared__ int waves[kOne / 64];
+  __shared__ int2 flags[kOne / 64];
   int mine = 0, live = 0;
   for (int64_t p = threadIdx.x; p < num_pages; p += kOne) mine += refs[p] > 0;
   block_scan(mine, waves, &live);
@@ -314,16 +327,16 @@ __global__ __launch_bounds__(kOne) void pages_compact_kernel(const int32_t* __re
     const int64_t p = p0 + threadIdx.x;
     const int ref = p < num_pages ? refs[p] : 0;
     const bool leaves = ref > 0 && p >= live, takes = p < num_pages && ref <= 0 && p < live;
-    int ns = 0, nd = 0;
-    const int rs = src + block_scan(leaves, waves, &ns), rd = dst + block_scan(takes, waves, &nd);
-    if (leaves) moves[2 * rs] = (int)p;
-    if (takes) moves[2 * rd + 1] = (int)p;
+    int2 n;
+    const int2 at = block_places(leaves, takes, flags, &n);
+    if (leaves) moves[2 * (src + at.x)] = (int)p;
+    if (takes) moves[2 * (dst + at.y) + 1] = (int)p;
     if (p < num_pages) {
       new_refs[p] = leaves ? 0 : ref;
       to[p] = (int)p;
     }
-    src += ns;
-    dst += nd;
+    src += n.x;
+    dst += n.y;
   }
   if (threadIdx.x == 0) {
     info[0] = src;
