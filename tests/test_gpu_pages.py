@@ -136,6 +136,17 @@ def test_copy(hip, dtype, planes, pages, shape):
         np.testing.assert_array_equal(y.numpy(), op.pages_copy(xh, moves, max(0, count)))
 
 
+def test_copy_past_the_caches(hip):
+    """Enough bytes for the copy's streaming form, in pages that are not whole pieces of it."""
+    xh = np.random.default_rng(83).integers(0, 1 << 16, (5, 400, 8, 64, 120), dtype=np.uint16)
+    x = Tensor(xh, dtype="bfloat16")
+    ids = np.random.default_rng(84).permutation(400)
+    moves = np.stack([ids[:150], ids[150:300]], 1)
+    F.pages_copy(x, i32(moves), i32([150]))
+    xh[:, moves[:, 1]] = xh[:, moves[:, 0]]
+    np.testing.assert_array_equal(x.handle.raw_bits(), xh)
+
+
 def test_a_beam_of_steps_replayed_from_a_graph(hip):
     """fork, reserve, copy of two steps (there and back between two sets of buffers) captured once, replayed with
     new parents, against the sequential form; what each row has written stays readable."""
