@@ -109,6 +109,7 @@ __device__ __forceinline__ void wave_best(Cand (&c)[N], int k, Cand* room, Cand*
     for (int j = lane; j < count; j += 64) {
       const Cand mine = room[j];
       int rank = 0;
+#pragma unroll 8
       for (int i = 0; i < count; ++i) rank += before(room[i], mine);
       if (rank < k) out[rank] = mine;
     }
@@ -261,7 +262,7 @@ __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __re
 }
 
 // A workgroup per group: the sums of its beams, then the k best of the runs' candidates, scored in float64.  Latency:
-// 5.3 us for one group of four beams, 8 for sixteen groups of eight (1216 candidates each).
+// 5.1 us for one group of four beams, 7.1 for sixteen groups of eight (1216 candidates each).
 constexpr int kMergeWaves = 16, kSlots = 2;
 __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
     const float2* __restrict__ sums, const uint64_t* __restrict__ keys, const float* __restrict__ scores,
@@ -273,6 +274,12 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
   __shared__ Cand best[kMergeWaves * kMaxK];
   const int g = blockIdx.x, lane = threadIdx.x & 63;
   const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int per = runs * k, all = beams * per;  // candidates (below 2^31: 64 beams, 2^18 runs, 64 each)
+  // the first candidates are under way beside the sums
+  uint64_t ahead[kSlots];
+#pragma unroll
+  for (int i = 0; i < kSlots; ++i)
+    ahead[i] = keys[(int64_t)g * all + min((w * kSlots + i) * 64 + lane, all - 1)];
   for (int b = w; b < beams; b += kMergeWaves) {
     const int row = g * beams + b;
     const double sc = (double)scores[row];
@@ -297,8 +304,6 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
     }
   }
   __syncthreads();
-  const int per = runs * k;
-  const int64_t all = (int64_t)beams * per;
   Cand* mine = best + w * k;
   for (int j = lane; j < k; j += 64) mine[j] = Cand{0, 0};
   for (int64_t i0 = 0; i0 < all; i0 += kMergeWaves * 64 * kSlots) {
@@ -308,13 +313,13 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
       const int64_t at = i0 + (int64_t)(w * kSlots + i) * 64 + lane;
       c[i] = Cand{0, 0};
       if (at < all) {
-        const int b = (int)(at / per), n = (int)(at - (int64_t)b * per);
+        const int b = (int)at / per, n = (int)at - b * per;
         if (done[b]) {
           if (n == 0) c[i] = Cand{order_bits(base[b] == base[b] ? base[b] : -(double)INFINITY), (int64_t)b * vocab + eos};
         } else if (base[b] != base[b]) {
           if (n < k && n < vocab) c[i] = Cand{order_bits(-(double)INFINITY), (int64_t)b * vocab + n};
         } else {
-          const uint64_t key = keys[(int64_t)(g * beams + b) * per + n];
+          const uint64_t key = i0 == 0 ? ahead[i] : keys[(int64_t)g * all + at];
           if (key != 0)
             c[i] = Cand{order_bits((double)order_value((uint32_t)(key >> 32)) + base[b]),
                         (int64_t)b * vocab + (int64_t)(0xffffffffu - (uint32_t)key)};
@@ -330,6 +335,7 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
     const Cand u = best[j];
     int rank = 0;
     if (u.hi != 0)
+#pragma unroll 4
       for (int i = threadIdx.x & 15; i < kMergeWaves * k; i += 16) rank += before(best[i], u);
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) rank += __shfl_xor(rank, off, 16);
