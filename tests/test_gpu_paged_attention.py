@@ -319,6 +319,21 @@ def test_padded_batches(hip, dtype, tokens, news, lens):
             compare(c, qh[:st[-1]], got[:st[-1]], st)
 
 
+@pytest.mark.parametrize("lens,news", [([1200], [500]), ([1200, 901], [290, 210])])
+def test_a_long_and_a_shorter_chunk(hip, lens, news):
+    """Tiles that fill more than half of the chip: their keys in two chunks of different length."""
+    c = Cache(75, "bfloat16", lens, 8, 64, 16)
+    check(c, 77, news, 80, max_query_len=max(news), max_kv_len=1200)
+
+
+def test_many_rows_of_pools_with_different_strides(hip):
+    """Keys with the heads inside the rows, values with the rows inside the heads."""
+    c = Cache(78, "bfloat16", [700, 90], 2, 128, 32)
+    c.k = F.permute(dev(np.ascontiguousarray(c.kh.transpose(0, 2, 1, 3)), "bfloat16"), (0, 2, 1, 3))
+    check(c, 79, [200, 1], 6)
+    check(c, 80, [1, 90], 6)
+
+
 def test_many_sequences(hip):
     """More sequences than are looked through at once, with gaps, lone tokens and chunks of many rows among them."""
     r = np.random.default_rng(67)
