@@ -135,16 +135,17 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_row_kernel(const
 }
 
 // A part of a launch of `tiles` tiles per kv head, of which `there` hold rows as far as can be told here: its keys in as
-// many equal chunks (multiples of 128 keys, `least` at least) as make no more than `most` workgroups with keys, and
-// partials (one per row and chunk) of no more than most_parts rows.  With f the part of the keys that the tiles do not
-// see on average, n chunks leave there (n (1 - f) + f) workgroups with keys.  Where that gives one chunk and a part of
-// another (`uneven`), a second, shorter one shares the places that one each would leave empty: 3000 tokens of 9000 keys
-// 269 -> 228 us, six chunks of up to 300 of 2600 96 -> 85; beside many workgroups of the other kind it loses (three
-// of up to 300 and 20 tokens 63 -> 76), and so do a third and later chunk like it.
-PagedPart part_of(const PagedCall& c, int64_t tiles, int64_t there, int least, int64_t most, int64_t most_parts, bool uneven) {
+// many equal chunks (multiples of 128 keys, `least` at least; up to `whole` keys in one) as make no more than `most`
+// workgroups with keys, and partials (one per row and chunk) of no more than most_parts rows.  With f the part of the
+// keys that the tiles do not see on average, n chunks leave there (n (1 - f) + f) workgroups with keys.  Where that
+// gives one chunk and a part of another (`uneven`), a second, shorter one shares the places that one each would leave
+// empty: 3000 tokens of 9000 keys 269 -> 222 us, six chunks of up to 300 of 2600 87 -> 70; beside many workgroups of
+// the other kind it loses (three of up to 300 and 20 tokens 63 -> 76), and so do a third and later chunk like it.
+PagedPart part_of(const PagedCall& c, int64_t tiles, int64_t there, int least, int whole, int64_t most, int64_t most_parts,
+                  bool uneven) {
   const int64_t len = c.pb.max_len, rows = (int64_t)c.pb.tokens * c.hq;
   if (there < 1) there = 1;
-  if (len <= least) return PagedPart{(int)(tiles * c.hkv), least, 1};
+  if (len <= whole) return PagedPart{(int)(tiles * c.hkv), whole, 1};
   const double f = c.causal ? 0.5 * (c.max_new < len ? c.max_new : len) / len : 0.0;
   double n = ((double)most / ((double)there * c.hkv) - f) / (1.0 - f);
   if (!uneven || n < 1.3 || n >= 2.0) n = (double)(int64_t)n;
@@ -198,10 +199,13 @@ int launch(const PagedCall& c) {
   // 512 keys of a tile at least: partials cost more than shorter chunks gain.  Beside a prompt's many rows, whose
   // workgroups take as long, few rows need no short chunks: partials of 2^18 rows at most.
   const int64_t places = cus * (waves == 8 ? 1 : 2);
-  const PagedPart few = part_of(c, few_tiles, few_there, 128, cus * (sizeof(T) == 4 && D == 128 ? 1 : 2),
-                                many_too ? 1 << 18 : INT64_MAX, !many_too);
+  // Few rows of up to 384 bf16 keys stay in one chunk: its third step costs less than the merge's launch (300 keys 7.8 us
+  // against 8.1, 200 keys 6.9 against 8.4; 450 keys 9.0 against 8.4; fp32 steps cost more: 200 keys 11.7 against 11.0).
+  const PagedPart few =
+      part_of(c, few_tiles, few_there, 128, sizeof(T) == 2 ? 384 : 128, cus * (sizeof(T) == 4 && D == 128 ? 1 : 2),
+              many_too ? 1 << 18 : INT64_MAX, !many_too);
   const PagedPart many =
-      part_of(c, many_tiles, many_tiles, 512, places, INT64_MAX, !few_too || few_there * c.hkv < places / 2);
+      part_of(c, many_tiles, many_tiles, 512, 512, places, INT64_MAX, !few_too || few_there * c.hkv < places / 2);
   const int few_chunks = few_too ? few.used : 1, many_chunks = many_too ? many.used : 1;
   const int chunks = few_chunks > many_chunks ? few_chunks : many_chunks;
   KH_REQUIRE(chunks <= 65535 && (int64_t)few.columns * few_chunks + (int64_t)many.columns * many_chunks <= INT32_MAX,
