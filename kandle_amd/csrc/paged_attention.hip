@@ -86,8 +86,8 @@ __global__ __launch_bounds__(256) void paged_merge_kernel(const float* __restric
   }
 }
 
-// Few rows (latency: 3.7 to 4.8 us): a workgroup per (token, query head); wave w sums chunks w, w + 4, ..., several loads in flight, and the
-// four sums are added in wave order.
+// Few rows (latency: 3.7 to 4.8 us): a workgroup per (token, query head); wave w sums chunks w, w + 4, ..., several
+// loads in flight, and the four sums are added in wave order.
 constexpr int kMergeWaves = 4;
 template <typename T, int D>
 __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_row_kernel(const float* __restrict__ part,

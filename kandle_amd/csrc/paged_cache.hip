@@ -160,8 +160,9 @@ __device__ __forceinline__ int2 block_places(bool a, bool b, int2* waves, int2* 
 // One workgroup.  A row that grows from len to len + count takes a new page for every table entry behind
 // its last page.  Of the rows that grow on one partly filled page, each gets a copy of it, also a new page, as long as
 // another row holds it, too: row after row, while the count less the copies before is above 1.  Nothing changes
-// unless all rows can grow.  64 rows, 64 sharing tails, in a pool of 685 pages: 6 us, a chain of four loads and three scans; the
-// free pages among the first kKept * 1024 keep their places from the count, which has to come first, to the writes.
+// unless all rows can grow.  64 rows that share tails in a pool of 685 pages: 6 us, a chain of four loads and three
+// scans; the free pages among the first kKept * 1024 keep their places from the count, which has to come first, to
+// the writes.
 constexpr int kKept = 4;
 __global__ __launch_bounds__(kOne) void pages_reserve_kernel(int32_t* __restrict__ table, int64_t stride,
                                                              int32_t* __restrict__ lens, int32_t* __restrict__ refs,
