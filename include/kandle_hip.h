@@ -586,11 +586,12 @@ int kh_pages_copy(void* pages, int64_t planes, int64_t num_pages, int64_t page_b
  *   score(g, b, t) = logits[g, b, t] - log(sum_t' exp logits[g, b, t']) + scores[g, b],
  * a NaN logit or score counting as -inf, and all continuations of a beam whose score or sum is not finite
  * being -inf.  With finished (int32 [groups, beams], may be NULL) a beam whose flag is not 0 has one
- * continuation, the token eos at an unchanged score.  The k best of each group in order (the larger score,
- * then the lower beam; inside a beam the larger logit, then the lower token): out_scores (fp32),
+ * continuation, the token eos at an unchanged score.  The k best of each group in order (the larger score in
+ * float64, then the lower beam, then the larger logit, then the lower token; the logits of a beam all of whose
+ * continuations are -inf count as equal): out_scores (fp32),
  * out_tokens, out_parents (the beam, int32) and out_finished (given with finished: the parent's flag, or the
  * token is eos), each [groups, k].  k <= 64, beams <= 64, k <= beams * vocab (with finished: k <= beams).
- * Candidates are compared in float64.  No result shares memory with an input.  Extends sample() (reference:
+ * No result shares memory with an input.  Extends sample() (reference:
  * packages/model-utils/src/sampling/index.ts:103-243) to several hypotheses. */
 int kh_beam_select(const void* logits, const int64_t* strides, const float* scores, const int32_t* finished, int64_t groups,
                    int64_t beams, int64_t vocab, int k, int64_t eos, float* out_scores, int32_t* out_tokens,

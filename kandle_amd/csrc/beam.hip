@@ -3,8 +3,9 @@
 //
 //   score(beam, token) = logits[beam, token] - log sum exp(logits[beam, :]) + scores[beam]
 // A finished beam has one continuation: itself, with the end token.  NaN, as a logit or a score, counts
-// as -inf.  Order: the larger score, then the lower beam, then the lower token.  Inside a beam the logits
-// decide, so only the k largest of each beam are scored, in float64.
+// as -inf.  Order: the larger score in float64, then the lower beam, then the larger logit, then the lower token.  A
+// beam's scores never fall as its logits grow (where its score so far is large, different logits make one score),
+// so inside a beam the logits decide, and only the k largest of each are scored.
 #include "paged.h"
 
 using namespace kh;
@@ -74,12 +75,15 @@ __device__ __forceinline__ uint32_t kth_lane(uint32_t top, int k) {
   return floor;
 }
 
-// A candidate of the merge: the larger `hi` (order bits of a float64 score) first, then the lower `at` (beam *
-// vocab + token).  hi 0: none.
+// A candidate of the merge: the larger `hi` (order bits of a float64 score) first, then the lower `at`: beam, inverted
+// order bits of the logit, and place among the beam's candidates, of which those of equal logits lie in the order of
+// their tokens (6, 32 and 24 bits: 64 beams of 2^18 runs of 64 candidates).  hi 0: none.
 struct Cand {
-  uint64_t hi;
-  int64_t at;
+  uint64_t hi, at;
 };
+__device__ __forceinline__ uint64_t cand_at(int beam, uint32_t logit_bits, int place) {
+  return (uint64_t)beam << 56 | (uint64_t)~logit_bits << 24 | (uint64_t)place;
+}
 __device__ __forceinline__ bool before(const Cand& a, const Cand& b) { return a.hi > b.hi || (a.hi == b.hi && a.at < b.at); }
 
 // The k best of a wave's candidates, N per lane in registers, in order to out[0 .. k) (LDS; none behind the
@@ -315,14 +319,13 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
       if (at < all) {
         const int b = (int)at / per, n = (int)at - b * per;
         if (done[b]) {
-          if (n == 0) c[i] = Cand{order_bits(base[b] == base[b] ? base[b] : -(double)INFINITY), (int64_t)b * vocab + eos};
-        } else if (base[b] != base[b]) {
-          if (n < k && n < vocab) c[i] = Cand{order_bits(-(double)INFINITY), (int64_t)b * vocab + n};
+          if (n == 0) c[i] = Cand{order_bits(base[b] == base[b] ? base[b] : -(double)INFINITY), cand_at(b, 0, 0)};
+        } else if (base[b] != base[b]) {  // (at -inf the logits count as equal: the first tokens)
+          if (n < k && n < vocab) c[i] = Cand{order_bits(-(double)INFINITY), cand_at(b, 0, n)};
         } else {
           const uint64_t key = i0 == 0 ? ahead[i] : keys[(int64_t)g * all + at];
-          if (key != 0)
-            c[i] = Cand{order_bits((double)order_value((uint32_t)(key >> 32)) + base[b]),
-                        (int64_t)b * vocab + (int64_t)(0xffffffffu - (uint32_t)key)};
+          const uint32_t logit = (uint32_t)(key >> 32);
+          if (key != 0) c[i] = Cand{order_bits((double)order_value(logit) + base[b]), cand_at(b, logit, n)};
         }
       }
     }
@@ -333,6 +336,9 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
   // the waves' best ranked among all, sixteen lanes to each
   for (int j = threadIdx.x / 16; j < kMergeWaves * k; j += kMergeWaves * 4) {
     const Cand u = best[j];
+    const int b = (int)(u.at >> 56), n = (int)(u.at & 0xffffff);
+    int t = done[b] ? eos : n;  // (a beam at -inf: its first tokens)
+    if (u.hi != 0 && !done[b] && base[b] == base[b]) t = (int)(0xffffffffu - (uint32_t)keys[(int64_t)g * all + b * per + n]);
     int rank = 0;
     if (u.hi != 0)
 #pragma unroll 4
@@ -340,7 +346,7 @@ __global__ __launch_bounds__(kMergeWaves * 64) void beam_merge_kernel(
 #pragma unroll
     for (int off = 8; off > 0; off >>= 1) rank += __shfl_xor(rank, off, 16);
     if (u.hi == 0 || rank >= k || (threadIdx.x & 15) != 0) continue;
-    const int b = (int)(u.at / vocab), t = (int)(u.at - (int64_t)b * vocab), o = g * k + rank;
+    const int o = g * k + rank;
     out_scores[o] = (float)order_value(u.hi);
     out_tokens[o] = t;
     out_parents[o] = b;

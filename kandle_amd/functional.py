@@ -189,8 +189,9 @@ def beam_select(logits: Tensor, scores: Tensor, k: Optional[int] = None, finishe
     eos_token_id, at their score.
 
     Returns (scores, tokens, parents, finished), each [groups, k] and best first: log_softmax(logits)[token] +
-    scores[parent], ties to the lower beam and token; finished is None without flags given.  out: the four results,
-    which share no memory with the inputs."""
+    scores[parent], compared in float64; where that is the same, the lower beam comes first, inside a beam the larger
+    logit, then the lower token.  finished is None without flags given.  out: the four results, which share no memory with
+    the inputs."""
     groups, beams = logits.shape[0], logits.shape[1]
     k = beams if k is None else int(k)
     if out is None:

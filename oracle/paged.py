@@ -145,13 +145,14 @@ def pages_copy(pages, moves, count):
 
 
 def beam_select(logits, scores, k, finished=None, eos=None):
-    """(scores float64, tokens, parents, finished) of each group, best first."""
+    """(scores float64, tokens, parents, finished) of each group, best first: the larger score in float64, then the
+    lower beam, then (at a finite score) the larger logit, then the lower token."""
     logits = np.asarray(logits, np.float64)
     groups, beams, vocab = logits.shape
     out = [np.zeros((groups, k)), np.zeros((groups, k), np.int64), np.zeros((groups, k), np.int64), np.zeros((groups, k), np.int64)]
     for g in range(groups):
         every = np.full((beams, vocab), -np.inf)
-        possible = np.ones((beams, vocab), bool)
+        possible, logit = np.ones((beams, vocab), bool), np.zeros((beams, vocab))
         for b in range(beams):
             base = float(scores[g, b])
             base = -np.inf if np.isnan(base) else base
@@ -163,9 +164,9 @@ def beam_select(logits, scores, k, finished=None, eos=None):
             m = x.max()
             if not np.isfinite(m) or not np.isfinite(base):
                 continue
-            every[b] = x - (m + np.log(np.exp(x - m).sum())) + base
-        order = sorted(np.flatnonzero(possible.reshape(-1)), key=lambda i: (-every.reshape(-1)[i], i)) if vocab * beams < 4096 else \
-            np.lexsort((np.arange(beams * vocab), -every.reshape(-1), ~possible.reshape(-1)))
+            every[b], logit[b] = x + (base - (m + np.log(np.exp(x - m).sum()))), x
+        beam, token = np.divmod(np.arange(beams * vocab), vocab)
+        order = np.lexsort((token, -logit.reshape(-1), beam, -every.reshape(-1), ~possible.reshape(-1)))
         for j, i in enumerate(order[:k]):
             out[0][g, j], out[1][g, j], out[2][g, j] = every.reshape(-1)[i], i % vocab, i // vocab
             if finished is not None:
