@@ -537,11 +537,18 @@ int kh_paged_attention(const void* q, const void* k_pages, const void* v_pages, 
  * whose row lies outside the table or in no page is not written.  `strides` (elements): k token, head;
  * v token, head; k_pages page, head, row; v_pages page, head, row.  Any d; rows on 16-byte boundaries
  * are copied 16 bytes at a time.  Replaces kvCache.update's slice copies (reference:
- * packages/model-utils/src/kv-cache.ts:164-212). */
+ * packages/model-utils/src/kv-cache.ts:164-212).
+ * The last n_b of L_b rows are taken to be the new tokens'.  If kh_pages_reserve lacked pages, L_b has not grown and
+ * they are cached rows, perhaps in pages that other sequences hold: a caller that has not looked at its `info` on
+ * the host hands it (device int32 [3]) to kh_paged_kv_write_reserved, which writes nothing then. */
 int kh_paged_kv_write(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
                       const int32_t* kv_lens, const int32_t* query_starts, int64_t tokens, int64_t batch, int hkv, int d,
                       int64_t num_pages, int64_t page_size, int64_t table_width, int64_t table_stride,
                       const int64_t* strides, int dtype);
+int kh_paged_kv_write_reserved(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
+                               const int32_t* kv_lens, const int32_t* query_starts, int64_t tokens, int64_t batch, int hkv,
+                               int d, int64_t num_pages, int64_t page_size, int64_t table_width, int64_t table_stride,
+                               const int64_t* strides, const int32_t* info, int dtype);
 
 /* Bookkeeping of the pages, on the device: page_refs [num_pages] (int32) counts the table entries that hold
  * each page; a page is free while its count is 0.  Table entries behind a sequence's last row are -1.
@@ -560,7 +567,8 @@ int kh_pages_fork(const int32_t* page_table, int64_t table_stride, const int32_t
  * the caller copies it before it writes there: moves [rows, 2] receives these (from, to) pairs in row
  * order and -1 behind them (kh_pages_copy takes them as they are); of several rows that grow on one page
  * nobody else holds, the last keeps it.  info [3]: the number of moves; the pages that were missing; the
- * rows that the table is too narrow for.  If either of the last two is not 0, nothing has changed.
+ * rows that the table is too narrow for.  If either of the last two is not 0, nothing has changed, and the new
+ * rows must not be written (kh_paged_kv_write_reserved).
  * At most 2048 rows, 2^30 cached rows in each and 2^31 table entries; no operands share memory. */
 int kh_pages_reserve(int32_t* page_table, int64_t table_stride, int32_t* kv_lens, int32_t* page_refs,
                      const int32_t* counts, int64_t rows, int64_t table_width, int64_t num_pages, int64_t page_size,

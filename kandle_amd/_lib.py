@@ -93,6 +93,8 @@ SIGNATURES = {
     "kh_paged_attention": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _i, _i, _i64, _i64, _i64, _i64, _i64p, _f,
                            _i, _i64, _i64, _i],
     "kh_paged_kv_write": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _i, _i64, _i64, _i64, _i64, _i64p, _i],
+    "kh_paged_kv_write_reserved": [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _i64, _i64, _i, _i, _i64, _i64, _i64, _i64, _i64p, _vp,
+                                   _i],
     "kh_pages_fork": [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _vp, _vp, _vp],
     "kh_pages_reserve": [_vp, _i64, _vp, _vp, _vp, _i64, _i64, _i64, _i64, _vp, _vp],
     "kh_pages_compact": [_vp, _i64, _vp, _i64, _i64, _i64, _vp, _vp, _vp, _i64, _vp],

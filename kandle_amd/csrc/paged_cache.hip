@@ -16,19 +16,21 @@ struct WriteStrides {
   int64_t kt, kh, vt, vh, kp, kph, kpr, vp, vph, vpr;
 };
 
-// A workgroup takes one token: its threads copy the heads' K and V rows in pieces of E.  6600 bf16 tokens of 8 heads
-// of 128: 11 us, 4.9 TB/s read and written, what a large copy reaches; one token of eight sequences: 2.8 us.
+// A workgroup takes one token: its threads copy the heads' K and V rows in pieces of E.  info (may be null): what
+// pages_reserve left; where that changed nothing, the new tokens' rows are other rows' places.  6600 bf16 tokens of 8
+// heads of 128: 11 us, 4.9 TB/s read and written, what a large copy reaches; one token of eight sequences: 2.8 us.
 template <typename E>
 __global__ __launch_bounds__(256) void paged_write_kernel(const E* __restrict__ K, const E* __restrict__ V,
                                                           E* __restrict__ KP, E* __restrict__ VP, PagedBatch pb, int hkv,
-                                                          int pieces, WriteStrides st) {
+                                                          int pieces, WriteStrides st, const int32_t* __restrict__ info) {
   const int t = blockIdx.x;
+  const bool lacking = info && (info[1] != 0 || info[2] != 0);
   const int b = pb.sequence_of(t);
   if (b < 0) return;
   const int pos = pb.len(b) - pb.count(b) + t - pb.first(b);
   if (pos < 0 || pos >= pb.max_len) return;
   const int id = pb.table[b * pb.table_stride + (pos >> pb.page_log)];
-  if (!pb.is_page(id)) return;
+  if (lacking || !pb.is_page(id)) return;
   const int slot = pos & ((1 << pb.page_log) - 1);
   for (int i = threadIdx.x; i < hkv * pieces; i += 256) {
     const int h = i / pieces, c = i - h * pieces;
@@ -413,11 +415,12 @@ __global__ __launch_bounds__(256) void pages_copy_kernel(uint8_t* __restrict__ p
 
 template <typename E>
 void launch_write(const void* k, const void* v, void* kp, void* vp, const PagedBatch& pb, int hkv, int d, int per,
-                  const int64_t* s) {
+                  const int64_t* s, const int32_t* info) {
   WriteStrides st{s[0], s[1], s[2], s[3], s[4], s[5], s[6], s[7], s[8], s[9]};
   int64_t* f = &st.kt;
   for (int i = 0; i < 10; ++i) f[i] /= per;
-  paged_write_kernel<E><<<pb.tokens, 256, 0, stream()>>>((const E*)k, (const E*)v, (E*)kp, (E*)vp, pb, hkv, d / per, st);
+  paged_write_kernel<E><<<pb.tokens, 256, 0, stream()>>>((const E*)k, (const E*)v, (E*)kp, (E*)vp, pb, hkv, d / per, st,
+                                                       info);
 }
 
 bool rows_ok(int64_t rows, int64_t width, int64_t stride, int64_t num_pages) {
@@ -438,6 +441,14 @@ int kh_paged_kv_write(const void* k, const void* v, void* k_pages, void* v_pages
                       const int32_t* kv_lens, const int32_t* query_starts, int64_t tokens, int64_t batch, int hkv, int d,
                       int64_t num_pages, int64_t page_size, int64_t table_width, int64_t table_stride,
                       const int64_t* strides, int dtype) {
+  return kh_paged_kv_write_reserved(k, v, k_pages, v_pages, page_table, kv_lens, query_starts, tokens, batch, hkv, d, num_pages,
+                                    page_size, table_width, table_stride, strides, nullptr, dtype);
+}
+
+int kh_paged_kv_write_reserved(const void* k, const void* v, void* k_pages, void* v_pages, const int32_t* page_table,
+                               const int32_t* kv_lens, const int32_t* query_starts, int64_t tokens, int64_t batch, int hkv,
+                               int d, int64_t num_pages, int64_t page_size, int64_t table_width, int64_t table_stride,
+                               const int64_t* strides, const int32_t* info, int dtype) {
   KH_REQUIRE_INIT();
   KH_REQUIRE(hkv > 0 && d > 0 && (int64_t)hkv * d <= INT32_MAX, "kh_paged_kv_write: bad extents (%d heads of %d)", hkv, d);
   KH_REQUIRE(dtype == KH_BF16 || dtype == KH_F32, "kh_paged_kv_write: unsupported dtype %d", dtype);
@@ -451,11 +462,11 @@ int kh_paged_kv_write(const void* k, const void* v, void* k_pages, void* v_pages
   bool wide = d % per == 0 && aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages);
   for (int i = 0; i < 10; ++i) wide = wide && strides[i] % per == 0;
   if (wide)
-    launch_write<uint4>(k, v, k_pages, v_pages, pb, hkv, d, per, strides);
+    launch_write<uint4>(k, v, k_pages, v_pages, pb, hkv, d, per, strides, info);
   else if (dtype == KH_BF16)
-    launch_write<uint16_t>(k, v, k_pages, v_pages, pb, hkv, d, 1, strides);
+    launch_write<uint16_t>(k, v, k_pages, v_pages, pb, hkv, d, 1, strides, info);
   else
-    launch_write<uint32_t>(k, v, k_pages, v_pages, pb, hkv, d, 1, strides);
+    launch_write<uint32_t>(k, v, k_pages, v_pages, pb, hkv, d, 1, strides, info);
   KH_CHECK_LAUNCH();
   return KH_OK;
 }

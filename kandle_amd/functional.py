@@ -124,11 +124,16 @@ def paged_attention(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_
 
 
 def paged_kv_write(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Tensor, page_table: Tensor,
-                   kv_lens: Tensor, query_starts: Optional[Tensor] = None) -> None:
+                   kv_lens: Tensor, query_starts: Optional[Tensor] = None, info: Optional[Tensor] = None) -> None:
     """Writes the new tokens' key and value rows [T, Hkv, D] into the pages that paged_attention will read
-    them from (same page_table, kv_lens and query_starts).  A row without a page is not written."""
+    them from (same page_table, kv_lens and query_starts).  A row without a page is not written.
+
+    The last rows that kv_lens counts are taken to be the new ones.  If pages_reserve lacked pages they are not: a program
+    that enqueues both without looking in between (a captured step) gives the info that it returns, and nothing
+    is written then."""
     _kernel(key, "paged_kv_write")(key.handle, value.handle, key_pages.handle, value_pages.handle, page_table.handle,
-                                   kv_lens.handle, query_starts.handle if query_starts is not None else None)
+                                   kv_lens.handle, query_starts.handle if query_starts is not None else None,
+                                   info.handle if info is not None else None)
 
 
 def pages_fork(page_table: Tensor, kv_lens: Tensor, page_refs: Tensor, parents: Tensor, out=None):
@@ -150,8 +155,8 @@ def pages_reserve(page_table: Tensor, kv_lens: Tensor, page_refs: Tensor, counts
     too, is replaced; its contents have to follow: pages_copy(pages, moves, info).
 
     Returns (moves int32 [rows, 2], info int32 [3]): pairs (from, to), and their number, the pages that were
-    missing and the rows that the table is too narrow for.  If any were, nothing has changed.  No two of the tensors
-    share memory."""
+    missing and the rows that the table is too narrow for.  If any were, nothing has changed, and the new rows must not
+    be written (paged_kv_write takes info).  No two of the tensors share memory."""
     if out is None:
         rows = page_table.shape[0]
         out = (_wrap(_new(page_table, (rows, 2))), _wrap(_new(page_table, (3,))))

@@ -64,6 +64,12 @@ class PagedKVCache:
     def page_refs(self) -> Tensor:
         return self.state[2]
 
+    @property
+    def reserve_info(self) -> Tensor:
+        """What the last reserve has left (int32 [3], on the device), for paged_kv_write: a step that lacked pages then
+        writes nothing over the cached rows."""
+        return self._info
+
     def layer(self, i: int):
         """(keys, values) of layer i: its two pools [pages, kv heads, page size, head dim]."""
         return self._pools[i]
@@ -84,7 +90,8 @@ class PagedKVCache:
 
     def enqueue_reserve(self, counts: Tensor) -> None:
         """reserve() for counts on the device (int32 [max_sequences]) and without the host's part: for a captured step,
-        whose caller advances `lens` at each replay (check_info() tells whether the pages sufficed)."""
+        whose caller advances `lens` at each replay, hands reserve_info to paged_kv_write, and asks check_info() after each
+        replay whether the pages sufficed."""
         F.pages_reserve(*self.state, counts, self.page_size, out=(self._moves, self._info))
         F.pages_copy(self.pages, self._moves, self._info)
 

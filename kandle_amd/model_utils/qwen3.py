@@ -458,7 +458,7 @@ class Qwen3ForCausalLM:
             v = Tensor(handle=HipTensorHandle.create_view(qkv.handle.storage, (T, Hkv, D), self.act, (nq + 2 * nkv, D, 1),
                                                           parts[2].offset))
             kp, vp = cache.layer(li)
-            F.paged_kv_write(k, v, kp, vp, cache.page_table, cache.kv_lens, starts)
+            F.paged_kv_write(k, v, kp, vp, cache.page_table, cache.kv_lens, starts, cache.reserve_info)
             o = F.paged_attention(q, kp, vp, cache.page_table, cache.kv_lens, starts, scale=self.scale,
                                   max_query_len=max_new, max_kv_len=max_len)
             out = F.view(o, (T, nq))

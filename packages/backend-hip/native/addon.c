@@ -719,7 +719,7 @@ FN(pagedAttention, 22)
   CALL(kh_paged_attention(q, kp, vp, o, (const int32_t*)pt, (const int32_t*)kl, (const int32_t*)qs, t, b, hq, hkv, d, np, ps,
                           tw, ts, st, (float)sc, causal, mq, mk, dt))
 /* pagedKvWrite(k, v, kPages, vPages, pageTable, kvLens, queryStarts | null, tokens, batch, hkv, d, numPages, pageSize,
-   tableWidth, tableStride, strides[10], dtype) */
+   tableWidth, tableStride, strides[10], dtype); pagedKvWriteReserved with the reserve's info | null at its end */
 FN(pagedKvWrite, 17)
   int64_t st[10];
   void* k = arg_ptr(A, 0); void* v = arg_ptr(A, 1); void* kp = arg_ptr(A, 2); void* vp = arg_ptr(A, 3);
@@ -729,6 +729,15 @@ FN(pagedKvWrite, 17)
   int dt = arg_int(A, 16);
   CALL(kh_paged_kv_write(k, v, kp, vp, (const int32_t*)pt, (const int32_t*)kl, (const int32_t*)qs, t, b, hkv, d, np, ps, tw,
                          ts, st, dt))
+FN(pagedKvWriteReserved, 18)
+  int64_t st[10];
+  void* k = arg_ptr(A, 0); void* v = arg_ptr(A, 1); void* kp = arg_ptr(A, 2); void* vp = arg_ptr(A, 3);
+  void* pt = arg_ptr(A, 4); void* kl = arg_ptr(A, 5); void* qs = arg_ptr(A, 6); int64_t t = arg_i64(A, 7);
+  int64_t b = arg_i64(A, 8); int hkv = arg_int(A, 9); int d = arg_int(A, 10); int64_t np = arg_i64(A, 11);
+  int64_t ps = arg_i64(A, 12); int64_t tw = arg_i64(A, 13); int64_t ts = arg_i64(A, 14); arg_list(A, 15, st, 10);
+  int dt = arg_int(A, 16); void* in = arg_ptr(A, 17);
+  CALL(kh_paged_kv_write_reserved(k, v, kp, vp, (const int32_t*)pt, (const int32_t*)kl, (const int32_t*)qs, t, b, hkv, d, np,
+                                  ps, tw, ts, st, (const int32_t*)in, dt))
 /* pagesFork(pageTable, tableStride, kvLens, pageRefs, parents, rows, tableWidth, numPages, newTable, newLens, newRefs) */
 FN(pagesFork, 11)
   void* pt = arg_ptr(A, 0); int64_t ts = arg_i64(A, 1); void* kl = arg_ptr(A, 2); void* rf = arg_ptr(A, 3);
@@ -782,7 +791,7 @@ static napi_value module_init(napi_env env, napi_value exports) {
       EXPORT(qkNormRope), EXPORT(flashAttention), EXPORT(flashAttentionSplit), EXPORT(flashAttentionMasked), EXPORT(decodeAttention),
       EXPORT(decodeAttentionNoalloc), EXPORT(gemm), EXPORT(gemmEx), EXPORT(gemmSwiglu), EXPORT(gemmQkNormRope), EXPORT(gemmQkNormRopeTable), EXPORT(ropeTable), EXPORT(gemmSplitCount),
       EXPORT(gemmSplitCountFor), EXPORT(gemmSplitkPartials), EXPORT(addRmsNorm), EXPORT(gemvFused), EXPORT(gemvSwiglu),
-      EXPORT(pagedAttention), EXPORT(pagedKvWrite), EXPORT(pagesFork), EXPORT(pagesReserve), EXPORT(pagesCompact), EXPORT(pagesCopy),
+      EXPORT(pagedAttention), EXPORT(pagedKvWrite), EXPORT(pagedKvWriteReserved), EXPORT(pagesFork), EXPORT(pagesReserve), EXPORT(pagesCompact), EXPORT(pagesCopy),
       EXPORT(beamSelect),
   };
   napi_define_properties(env, exports, sizeof(d) / sizeof(d[0]), d);

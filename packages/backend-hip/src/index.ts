@@ -745,10 +745,11 @@ function pagedAttention(q: HipTensorHandle, kPages: HipTensorHandle, vPages: Hip
                        q.kh);
 }
 
-// paged_kv_write(key, value, keyPages, valuePages, pageTable, kvLens, queryStarts | null): the new tokens' rows
-// [tokens, Hkv, D] into their pages.
+// paged_kv_write(key, value, keyPages, valuePages, pageTable, kvLens, queryStarts | null, info?): the new tokens' rows
+// [tokens, Hkv, D] into their pages, unless info, which pages_reserve left, says that they have no room.
 function pagedKvWrite(k: HipTensorHandle, v: HipTensorHandle, kPages: HipTensorHandle, vPages: HipTensorHandle,
-                      table: HipTensorHandle, kvLens: HipTensorHandle, queryStarts: HipTensorHandle | null): void {
+                      table: HipTensorHandle, kvLens: HipTensorHandle, queryStarts: HipTensorHandle | null,
+                      info?: HipTensorHandle): void {
   sameFloat('paged_kv_write', [k, v, kPages, vPages]);
   const pools = poolStrides('paged_kv_write', kPages, vPages);
   const hkv = kPages.shape[1], D = kPages.shape[3], T = k.shape[0];
@@ -757,9 +758,10 @@ function pagedKvWrite(k: HipTensorHandle, v: HipTensorHandle, kPages: HipTensorH
   const t = pageTableOf('paged_kv_write', table);
   int32Operand('paged_kv_write', 'kvLens', kvLens, [t[0]]);
   if (queryStarts !== null) int32Operand('paged_kv_write', 'queryStarts', queryStarts, [t[0] + 1]);
-  addon.pagedKvWrite(k.ptr, v.ptr, kPages.ptr, vPages.ptr, table.ptr, kvLens.ptr,
-                     queryStarts === null ? null : queryStarts.ptr, T, t[0], hkv, D, kPages.shape[0], kPages.shape[2], t[1],
-                     t[2], st.concat(pools), k.kh);
+  if (info !== undefined) int32Operand('paged_kv_write', 'info', info, [3]);
+  addon.pagedKvWriteReserved(k.ptr, v.ptr, kPages.ptr, vPages.ptr, table.ptr, kvLens.ptr,
+                             queryStarts === null ? null : queryStarts.ptr, T, t[0], hkv, D, kPages.shape[0], kPages.shape[2],
+                             t[1], t[2], st.concat(pools), k.kh, info === undefined ? null : info.ptr);
 }
 
 // pages_fork(pageTable, kvLens, pageRefs, parents, newTable, newLens, newRefs): rows follow their parents.
