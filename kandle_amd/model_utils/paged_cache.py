@@ -45,6 +45,7 @@ class PagedKVCache:
         self.state = self._new_state()
         self._other = self._new_state()
         self.lens = np.zeros(max_sequences, np.int64)
+        self._unchecked = 0   # reserves whose success the host has not looked at
         self._moves = F.zeros((max_sequences, 2), "int32")
         self._info = F.zeros((3,), "int32")
 
@@ -96,23 +97,37 @@ class PagedKVCache:
         F.pages_copy(self.pages, self._moves, self._info)
 
     def check_info(self) -> None:
-        """Raises if the last reserve lacked pages (waits for the device)."""
+        """Raises if the last reserve lacked pages, or one before it that reserve(check=False) left unchecked (waits for
+        the device).  `lens` are then the device's: a reserve that lacked pages has changed nothing."""
         _, missing, too_long = self._info.numpy().tolist()
-        if missing or too_long:
-            raise RuntimeError(f"PagedKVCache: {missing} pages are missing ({self.num_pages} of {self.page_size} rows in all)"
-                               if missing else f"PagedKVCache: {too_long} rows are too long for the page table")
+        unchecked, self._unchecked = self._unchecked, 0
+        if not missing and not too_long and unchecked < 2:
+            return
+        lens = self.kv_lens.numpy().astype(np.int64)   # (info speaks of the last reserve alone)
+        same, self.lens = np.array_equal(lens, self.lens), lens
+        if missing:
+            raise RuntimeError(f"PagedKVCache: {missing} pages are missing ({self.num_pages} of {self.page_size} rows in all)")
+        if too_long:
+            raise RuntimeError(f"PagedKVCache: {too_long} rows are too long for the page table")
+        if not same:
+            raise RuntimeError(f"PagedKVCache: pages were missing for a reserve before the last ({self.num_pages} of "
+                               f"{self.page_size} rows in all)")
 
     def reserve(self, counts: Sequence[int], check: bool = True) -> None:
         """Makes room for counts[s] new rows behind each sequence's cached ones, which kv_lens then includes.  Pages
         that a sequence grows into are its own afterwards.  check: raise if the pool has too few free pages (nothing
-        has changed then); without it the caller looks at check_info() later."""
+        has changed then); without it the caller hands reserve_info to what it enqueues (paged_kv_write) and calls
+        check_info() later, until which `lens` counts on the pages."""
+        if check and self._unchecked:
+            self.check_info()   # before anything is enqueued behind it
         n = self._check_counts(counts)
         t = Tensor(n.astype(np.int32), dtype="int32")
         self.enqueue_reserve(t)
         t.dispose()
+        self.lens += n
+        self._unchecked += 1
         if check:
             self.check_info()
-        self.lens += n
 
     def enqueue_fork(self, parents: Tensor) -> None:
         """fork() for parents on the device, without the host's part."""

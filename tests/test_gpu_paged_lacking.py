@@ -114,6 +114,41 @@ def test_a_model_step_that_lacks_pages_loses_no_row(hip):
     model.dispose()
 
 
+def test_the_hosts_lengths_are_the_devices_after_a_reserve_that_lacked_pages(hip):
+    cache = full_cache(1)
+    cache.reserve([1, 0, 0], check=False)     # the free page
+    cache.check_info()
+    assert cache.lens.tolist() == cache.kv_lens.numpy().tolist() == [25, 24, 0]
+    cache.reserve([8, 1, 5], check=False)     # two pages that are not there
+    with pytest.raises(RuntimeError, match="2 pages are missing"):
+        cache.check_info()
+    assert cache.lens.tolist() == cache.kv_lens.numpy().tolist() == [25, 24, 0]
+    cache.reserve([7, 8, 0])                  # the tails' room
+    assert cache.lens.tolist() == cache.kv_lens.numpy().tolist() == [32, 32, 0]
+    with pytest.raises(RuntimeError, match="1 pages are missing"):
+        cache.reserve([0, 0, 3])
+    assert cache.lens.tolist() == [32, 32, 0]
+    cache.dispose()
+
+
+@pytest.mark.parametrize("check", [False, True])
+def test_a_reserve_that_lacked_pages_before_the_last_is_found(hip, check):
+    """info is the last reserve's; one before it, which nobody looked at, shows in the lengths."""
+    cache = full_cache(1)
+    cache.reserve([0, 0, 17], check=False)    # two pages of one
+    cache.reserve([1, 0, 0], check=False)     # the free one
+    with pytest.raises(RuntimeError, match="before the last"):
+        cache.reserve([1, 0, 0], check=True) if check else cache.check_info()
+    assert cache.lens.tolist() == cache.kv_lens.numpy().tolist() == [25, 24, 0]
+    cache.check_info()
+    cache.reserve([1, 1, 0], check=False)
+    cache.reserve([1, 1, 0], check=False)
+    cache.fork([1, 0, 0])
+    cache.check_info()
+    assert cache.lens.tolist() == cache.kv_lens.numpy().tolist() == [26, 27, 27]
+    cache.dispose()
+
+
 SCRIPT = r"""
 const m = require(process.argv[1]), addon = require(process.argv[2]);
 m.HipBackend.create(0).then((b) => {
