@@ -524,7 +524,7 @@ int kh_gemv_swiglu(int prologue, const void* x, const void* norm_w, float eps, c
  * or behind it are not seen); both only size the launch, and INT64_MAX is always right.  Rows of o
  * behind query_starts[batch] stay as they were.  `strides` (elements): q token, head; k page, head, row;
  * v page, head, row; o token, head.  d 64 or 128, dtype KH_BF16 or KH_F32 (fp32 arithmetic throughout),
- * q, pools and o 16-byte aligned with strides in 16-byte units.
+ * q, pools and o 16-byte aligned with strides in 16-byte units.  o shares no memory with an input.
  * Extends flash_attention (reference: packages/types/src/backend/register.ts:102-109) to chunks behind a
  * cached prefix and to ragged batches. */
 int kh_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,
@@ -536,7 +536,8 @@ int kh_paged_attention(const void* q, const void* k_pages, const void* v_pages, 
 /* Writes the new tokens' k and v rows ([tokens, hkv, d], token and head strides) into their pages.  A token
  * whose row lies outside the table or in no page is not written.  `strides` (elements): k token, head;
  * v token, head; k_pages page, head, row; v_pages page, head, row.  Any d; rows on 16-byte boundaries
- * are copied 16 bytes at a time.  Replaces kvCache.update's slice copies (reference:
+ * are copied 16 bytes at a time.  The pools share no memory with an input or each other (but for one pool that
+ * k == v is written to as both).  Replaces kvCache.update's slice copies (reference:
  * packages/model-utils/src/kv-cache.ts:164-212).
  * The last n_b of L_b rows are taken to be the new tokens'.  If kh_pages_reserve lacked pages, L_b has not grown and
  * they are cached rows, perhaps in pages that other sequences hold: a caller that has not looked at its `info` on

@@ -375,9 +375,11 @@ int kh_beam_select(const void* logits, const int64_t* strides, const float* scor
   if (groups == 0) return KH_OK;
   KH_REQUIRE(logits && strides && scores && out_scores && out_tokens && out_parents, "kh_beam_select: null pointer");
   const int64_t rows = groups * beams;
+  const int64_t size = dtype == KH_BF16 ? 2 : 4;
   KH_REQUIRE(!overlap({ints(out_scores, groups * k), ints(out_tokens, groups * k), ints(out_parents, groups * k),
                        ints(out_finished, groups * k)},
-                      {ints(scores, rows), ints(finished, rows)}),
+                      {ints(scores, rows), ints(finished, rows),
+                       Span(logits, size * vocab, groups, size * strides[0], beams, size * strides[1])}),
              "kh_beam_select: the results must not share memory with the inputs or each other");
   const int shift = (dtype == KH_BF16 ? 8 : 4) - 1;  // a row may start this far inside a 16-byte block
   const int runs = (int)((vocab + shift + kRun - 1) / kRun);

@@ -1,9 +1,8 @@
 // Shared by the kernels of the paged KV cache: where a token of a ragged batch sits.
 #pragma once
 
-#include <initializer_list>
-
 #include "common.h"
+#include "spans.h"
 
 namespace kh {
 
@@ -175,30 +174,6 @@ struct PagedPart {
 void launch_paged_tiles(const PagedCall& c, int d, int waves, const PagedPart& many, int chunks, float* part);
 void launch_paged_mixed(const PagedCall& c, int d, int few_rows, const PagedPart& many, const PagedPart& few, int chunks,
                         float* part);
-
-// Whether any of the memory that a call writes overlaps what it reads, or other memory that it writes.
-struct Span {
-  const void* at;
-  int64_t bytes;
-};
-inline bool overlap(std::initializer_list<Span> written, std::initializer_list<Span> read) {
-  auto meet = [](const Span& a, const Span& b) {
-    const uintptr_t x = (uintptr_t)a.at, y = (uintptr_t)b.at;
-    return x != 0 && y != 0 && a.bytes > 0 && b.bytes > 0 && x < y + (uint64_t)b.bytes && y < x + (uint64_t)a.bytes;
-  };
-  for (const Span& a : written) {
-    for (const Span& b : read)
-      if (meet(a, b)) return true;
-    for (const Span& b : written)
-      if (&a < &b && meet(a, b)) return true;
-  }
-  return false;
-}
-// Of n int32 values; of a page table.
-inline Span ints(const void* at, int64_t n) { return Span{at, 4 * n}; }
-inline Span table_span(const int32_t* at, int64_t stride, int64_t rows, int64_t width) {
-  return Span{at, rows == 0 || width == 0 ? 0 : 4 * ((rows - 1) * stride + width)};
-}
 
 inline int log2_of(int64_t v) {
   int n = 0;

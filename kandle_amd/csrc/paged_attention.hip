@@ -306,6 +306,15 @@ int kh_paged_attention(const void* q, const void* k_pages, const void* v_pages, 
   // sixteen rows of a page are addressed with 32-bit byte offsets
   KH_REQUIRE(strides[4] >= 0 && strides[4] <= (1 << 24) && strides[7] >= 0 && strides[7] <= (1 << 24),
              "kh_paged_attention: the pages' row strides must be from 0 to 2^24");
+  const int64_t size = dtype == KH_BF16 ? 2 : 4, run = size * d;
+  auto rows = [&](const void* at, const int64_t* st) { return Span(at, run, tokens, size * st[0], hq, size * st[1]); };
+  auto pool = [&](const void* at, const int64_t* st) {
+    return Span(at, run, num_pages, size * st[0], hkv, size * st[1], page_size, size * st[2]);
+  };
+  KH_REQUIRE(!overlap({rows(o, strides + 8)},
+                      {rows(q, strides), pool(k_pages, strides + 2), pool(v_pages, strides + 5),
+                       table_span(page_table, table_stride, batch, table_width), ints(kv_lens, batch), ints(query_starts, batch + 1)}),
+             "kh_paged_attention: the output must not share memory with the inputs");
   c.q = q;
   c.k = k_pages;
   c.v = v_pages;

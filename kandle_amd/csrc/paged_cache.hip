@@ -458,7 +458,21 @@ int kh_paged_kv_write_reserved(const void* k, const void* v, void* k_pages, void
   if (rc != KH_OK) return rc;
   if (tokens == 0 || batch == 0 || num_pages == 0 || table_width == 0) return KH_OK;
   KH_REQUIRE(k && v && k_pages && v_pages && page_table && kv_lens && strides, "kh_paged_kv_write: null pointer");
-  const int size = dtype == KH_BF16 ? 2 : 4, per = 16 / size;
+  const int64_t size = dtype == KH_BF16 ? 2 : 4;
+  const int per = (int)(16 / size);
+  auto rows = [&](const void* at, const int64_t* s) { return Span(at, size * d, tokens, size * s[0], hkv, size * s[1]); };
+  auto pool = [&](const void* at, const int64_t* s) {
+    return Span(at, size * d, num_pages, size * s[0], hkv, size * s[1], page_size, size * s[2]);
+  };
+  const Span keys = rows(k, strides), values = rows(v, strides + 2), kp = pool(k_pages, strides + 4), vp = pool(v_pages, strides + 7),
+             table = table_span(page_table, table_stride, batch, table_width), lens = ints(kv_lens, batch),
+             starts = ints(query_starts, batch + 1), left = ints(info, 3);
+  // (one pool may be keys and values at once where one tensor is, too)
+  bool one = k == v && k_pages == v_pages && strides[0] == strides[2] && strides[1] == strides[3];
+  for (int i = 0; i < 3; ++i) one = one && strides[4 + i] == strides[7 + i];
+  KH_REQUIRE(!overlap({kp}, {keys, values, table, lens, starts, left}) && !overlap({vp}, {keys, values, table, lens, starts, left}) &&
+                 (one || apart(kp, vp)),
+             "kh_paged_kv_write: the pages must not share memory with the inputs or each other");
   bool wide = d % per == 0 && aligned16(k) && aligned16(v) && aligned16(k_pages) && aligned16(v_pages);
   for (int i = 0; i < 10; ++i) wide = wide && strides[i] % per == 0;
   if (wide)
@@ -570,6 +584,9 @@ int kh_pages_copy(void* pages, int64_t planes, int64_t num_pages, int64_t page_b
   KH_REQUIRE(page_bytes % 16 == 0 && aligned16(pages), "kh_pages_copy: pages must be 16-byte aligned, of a multiple of 16 bytes");
   if (planes == 0 || num_pages == 0 || page_bytes == 0 || max_moves == 0) return KH_OK;
   KH_REQUIRE(pages && moves && info, "kh_pages_copy: null pointer");
+  KH_REQUIRE(!overlap({Span(pages, page_bytes, num_pages, page_bytes, planes, num_pages * page_bytes)},
+                      {ints(moves, 2 * max_moves), ints(info, 1)}),
+             "kh_pages_copy: the pages must not share memory with the moves");
   const int64_t items = max_moves * planes * ((page_bytes + kPiece - 1) / kPiece), most = 8 * (int64_t)cu_count();
   pages_copy_kernel<<<(unsigned)(items < most ? items : most), 256, 0, stream()>>>(
       (uint8_t*)pages, planes, num_pages * page_bytes, page_bytes, (int)num_pages, moves, (int)max_moves, info);

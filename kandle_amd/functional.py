@@ -112,7 +112,7 @@ def paged_attention(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_
 
     max_query_len and max_kv_len, upper bounds of the new tokens and cached rows of a sequence, keep the launch
     small; tokens and rows beyond them are left out.  Rows of `out` behind the last sequence stay as they
-    were (a new result's are undefined)."""
+    were (a new result's are undefined); it shares no memory with an input."""
     if scale is None:
         scale = 1.0 / math.sqrt(query.shape[-1])
     output = out.handle if out is not None else _new(query, query.shape)
@@ -126,7 +126,8 @@ def paged_attention(query: Tensor, key_pages: Tensor, value_pages: Tensor, page_
 def paged_kv_write(key: Tensor, value: Tensor, key_pages: Tensor, value_pages: Tensor, page_table: Tensor,
                    kv_lens: Tensor, query_starts: Optional[Tensor] = None, info: Optional[Tensor] = None) -> None:
     """Writes the new tokens' key and value rows [T, Hkv, D] into the pages that paged_attention will read
-    them from (same page_table, kv_lens and query_starts).  A row without a page is not written.
+    them from (same page_table, kv_lens and query_starts).  A row without a page is not written.  The pools share no
+    memory with the rows, nor with each other unless key and value are one tensor, too.
 
     The last rows that kv_lens counts are taken to be the new ones.  If pages_reserve lacked pages they are not: a program
     that enqueues both without looking in between (a captured step) gives the info that it returns, and nothing

@@ -1207,7 +1207,7 @@ def paged_attention(query, key_pages, value_pages, page_table, kv_lens, query_st
               _NO_LIMIT if max_query_len is None else max_query_len, _NO_LIMIT if max_kv_len is None else max_kv_len, dtype)
 
 
-def _paged_kv_write_plan(key, value, key_pages, value_pages, table, kv_lens, query_starts, info):
+def _paged_kv_write_plan(key, value, key_pages, value_pages, table, kv_lens, query_starts):
     dt = key.dtype
     if dt not in (FLOAT32, BFLOAT16) or value.dtype != dt or key_pages.dtype != dt or value_pages.dtype != dt:
         raise TypeError(f"paged_kv_write: rows and pages must share float32 or bfloat16, got {dt}, {value.dtype}, "
@@ -1219,18 +1219,19 @@ def _paged_kv_write_plan(key, value, key_pages, value_pages, table, kv_lens, que
     if value.shape[0] != tokens:
         raise ValueError(f"paged_kv_write: key has {tokens} tokens, value {value.shape[0]}")
     B, width, stride = _sequences("paged_kv_write", table, kv_lens, query_starts, tokens)
-    if info is not None:
-        _int32("paged_kv_write", "info", info, (3,))
     return tokens, B, hkv, d, n_pages, page, width, stride, _lib.i64_array(st + pools), key.kh_dtype
 
 
 def paged_kv_write(key, value, key_pages, value_pages, page_table, kv_lens, query_starts, info=None) -> None:
     """The new tokens' rows key / value [tokens, Hkv, D] into their pages, unless info, which pages_reserve left, says that
     they have no room (kh_paged_kv_write_reserved)."""
-    *plan, dtype = _plan(_paged_kv_write_plan, key, value, key_pages, value_pages, page_table, kv_lens, query_starts, info)
-    _lib.call("kh_paged_kv_write_reserved", key.data_ptr(), value.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(),
-              page_table.data_ptr(), kv_lens.data_ptr(), None if query_starts is None else query_starts.data_ptr(), *plan,
-              None if info is None else info.data_ptr(), dtype)
+    plan = _plan(_paged_kv_write_plan, key, value, key_pages, value_pages, page_table, kv_lens, query_starts)
+    entry = "kh_paged_kv_write"
+    if info is not None:
+        _int32("paged_kv_write", "info", info, (3,))
+        entry, plan = "kh_paged_kv_write_reserved", (*plan[:-1], info.data_ptr(), plan[-1])
+    _lib.call(entry, key.data_ptr(), value.data_ptr(), key_pages.data_ptr(), value_pages.data_ptr(), page_table.data_ptr(),
+              kv_lens.data_ptr(), None if query_starts is None else query_starts.data_ptr(), *plan)
 
 
 def _page_refs(name: str, page_refs) -> int:
