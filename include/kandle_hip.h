@@ -523,8 +523,10 @@ int kh_gemv_swiglu(int prologue, const void* x, const void* norm_w, float eps, c
  * bound of n_b (tokens j >= max_query_len are not computed); max_kv_len: an upper bound of L_b (rows at
  * or behind it are not seen); both only size the launch, and INT64_MAX is always right.  Rows of o
  * behind query_starts[batch] stay as they were.  `strides` (elements): q token, head; k page, head, row;
- * v page, head, row; o token, head.  d 64 or 128, dtype KH_BF16 or KH_F32 (fp32 arithmetic throughout),
- * q, pools and o 16-byte aligned with strides in 16-byte units.  o shares no memory with an input.
+ * v page, head, row; o token, head.  d 64 or 128, dtype KH_BF16 or KH_F32, q, pools
+ * and o 16-byte aligned with strides in 16-byte units.  Scores, softmax and sums are fp32; KH_BF16 rounds the result, and
+ * the probabilities: to 2^-8 in sequences of more than 256 new tokens times hq / hkv, as kh_flash_attention does, to 2^-16 in
+ * others.  o shares no memory with an input.
  * Extends flash_attention (reference: packages/types/src/backend/register.ts:102-109) to chunks behind a
  * cached prefix and to ragged batches. */
 int kh_paged_attention(const void* q, const void* k_pages, const void* v_pages, void* o, const int32_t* page_table,

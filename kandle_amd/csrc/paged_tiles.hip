@@ -7,6 +7,8 @@
 //   and 3 of the key swapped so that S^T leaves P in the operand layout of the second product, V read
 //   transposed (ds_read_b64_tr_b16), the softmax relative to a reference that the accumulators start from
 //   (flash_tiles.h) -- the products of the contiguous prefill kernel.
+// P is rounded to bf16 once for the second product, as there: these tiles are bound by their products, of which a second
+// part of P would make half as many again (2-norm error 2.3e-3, of which the result's rounding is 1.7e-3).
 // What differs is where rows come from: 16 keys lie in one page, the threads of a wave that load together
 // read inside one such block, so a block's place is a lane's value read as scalars (one lane per block, worked
 // out for 1024 keys at once), and its buffer range ends with the page's rows that the tile sees (others, and

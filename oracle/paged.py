@@ -174,3 +174,23 @@ def beam_select(logits, scores, k, finished=None, eos=None):
             if finished is not None:
                 out[3][g, j] = int(bool(finished[g, i // vocab]) or i % vocab == eos)
     return out[0], out[1], out[2], (out[3] if finished is not None else None)
+
+
+def attention_spread(q, k_pages, v_pages, table, kv_lens, starts=None, scale=None, causal=True):
+    """(sum p^2 v^2, sum p^2) of each row of paged_attention: what independent roundings of p add up to, squared."""
+    q, kp, vp = (np.asarray(x, np.float64) for x in (q, k_pages, v_pages))
+    pages, hkv, page, d = kp.shape
+    scale = 1.0 / np.sqrt(d) if scale is None else scale
+    pv, pp = np.zeros(q.shape), np.zeros(q.shape[:2])
+    for b, t0, n, length in _sequences(len(q), kv_lens, starts):
+        for j in range(n):
+            rows = np.arange(max(0, min(length - n + j + 1 if causal else length, table.shape[1] * page)))
+            rows = rows[(table[b, rows // page] >= 0) & (table[b, rows // page] < pages)]
+            if not len(rows):
+                continue
+            k, v = (np.repeat(x[table[b, rows // page], :, rows % page], q.shape[1] // hkv, 1) for x in (kp, vp))
+            s = scale * np.einsum("hd,khd->kh", q[t0 + j], k)
+            p = np.exp(s - s.max(0))
+            p /= p.sum(0)
+            pv[t0 + j], pp[t0 + j] = np.einsum("kh,khd->hd", p * p, v * v), (p * p).sum(0)
+    return pv, pp
