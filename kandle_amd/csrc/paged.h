@@ -39,8 +39,8 @@ struct PagedBatch {
       below += n;
       if (n < 256) break;
     }
-    const int b = below - 1;
-    return b >= 0 && t < first(b) + count(b) ? b : -1;
+    const int b = below - 1;  // (where the starts do not grow, t may lie before its first token)
+    return b >= 0 && t >= first(b) && t < first(b) + count(b) ? b : -1;
   }
 };
 
@@ -73,7 +73,8 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& pb, int x, int G, in
     constexpr int PER = 4;
     const int lane = threadIdx.x & 63;
     for (int b0 = 0; b0 < pb.batch; b0 += 64 * PER) {
-      int start[PER + 1], len[PER], tiles[PER], sum = 0;
+      int start[PER + 1], len[PER], tiles[PER];
+      uint32_t sum = 0;  // (starts that overlap can make it pass 2^32; what comes out is looked at below)
 #pragma unroll
       for (int k = 0; k <= PER; ++k) start[k] = min(max(pb.starts[min(b0 + PER * lane + k, pb.batch)], 0), pb.tokens);
 #pragma unroll
@@ -82,18 +83,18 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& pb, int x, int G, in
       for (int k = 0; k < PER; ++k) {
         const int n = min(max(0, start[k + 1] - start[k]), max_new);
         tiles[k] = n * G > above && n * G <= upto ? (n * G + rows - 1) / rows : 0;
-        sum += tiles[k];
+        sum += (uint32_t)tiles[k];
       }
-      int inc = sum;
+      uint32_t inc = sum;
 #pragma unroll
       for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(inc, o, 64);
+        const uint32_t u = __shfl_up(inc, o, 64);
         if (lane >= o) inc += u;
       }
-      const int all = __builtin_amdgcn_readlane(inc, 63);
+      const int all = __builtin_amdgcn_readlane((int)inc, 63);
       if (at < all) {
-        const int who = __ffsll((unsigned long long)__ballot(inc > at)) - 1;
-        int rest = at - (inc - sum), which = 0;  // in lane `who`: its sequence, and the tile there
+        const int who = __ffsll((unsigned long long)__ballot((int)inc > at)) - 1;
+        int rest = (int)((uint32_t)at - (inc - sum)), which = 0;  // in lane `who`: its sequence, and the tile there
         bool found = false;
 #pragma unroll
         for (int k = 0; k < PER; ++k) {
@@ -104,7 +105,7 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& pb, int x, int G, in
             t.n = max(0, start[k + 1] - start[k]);
             t.len = len[k];
           }
-          if (!found) rest -= tiles[k];
+          if (!found) rest = (int)((uint32_t)rest - (uint32_t)tiles[k]);
         }
         t.b = b0 + PER * who + __builtin_amdgcn_readlane(which, who);
         at = __builtin_amdgcn_readlane(rest, who);
@@ -113,11 +114,11 @@ __device__ __forceinline__ Tile find_tile(const PagedBatch& pb, int x, int G, in
         t.len = __builtin_amdgcn_readlane(t.len, who);
         break;
       }
-      at -= all;
+      at = (int)((uint32_t)at - (uint32_t)all);
     }
     if (t.b < 0) return t;
   }
-  t.row0 = at * rows;
+  t.row0 = (int)((uint32_t)at * (uint32_t)rows);
   t.rows = min(t.n, max_new) * G;
   if (t.row0 < 0 || t.row0 >= t.rows) t.b = -1;  // (starts that overlap can claim more tiles than there are)
   return t;
