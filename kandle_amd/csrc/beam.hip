@@ -141,9 +141,10 @@ __device__ __forceinline__ void wave_best(Cand (&c)[N], int k, Cand* room, Cand*
 // exponentials relative to it, and the k largest in order.  Rows may start anywhere: the lanes' 16-byte loads
 // lie on the 16-byte grid of the memory, and those that cross a row's ends are made value by value.
 //
-// Bound by the vector ALU (13.5 instructions per logit, four of them the exponential's) and the selection's chain: 128
-// rows of 151936 bf16 logits, of which a quarter have finished, 16 us (29 MB); four fp32 rows 7.7.  Runs of twice the
-// length in as many registers are slower (22.4 -> 25.3 us a call): fewer waves hide the chain.
+// Bound by the chain load -> maximum -> threshold -> ranking of waves that all start together: 128 rows of 151936 bf16
+// logits, of which a quarter have finished, 16 us (29 MB), in which a wave waits 60 % of its time and the vector ALU (13.5
+// instructions per logit, four of them the exponential's) is busy for half; four fp32 rows, 76 workgroups, 7.8.  Runs of
+// twice the length in as many registers are slower (22.4 -> 25.3 us a call): fewer waves hide the chain.
 constexpr int kPer = 32, kRunWaves = 4, kRun = kPer * 64 * kRunWaves;
 template <typename T>
 __global__ __launch_bounds__(kRunWaves * 64) void beam_runs_kernel(const T* __restrict__ logits, int64_t sg, int64_t sb,

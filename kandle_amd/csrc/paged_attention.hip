@@ -139,8 +139,10 @@ __global__ __launch_bounds__(kMergeWaves * 64) void paged_merge_row_kernel(const
 // workgroups with keys, and partials (one per row and chunk) of no more than most_parts rows.  With f the part of the
 // keys that the tiles do not see on average, n chunks leave there (n (1 - f) + f) workgroups with keys.  Where that
 // gives one chunk and a part of another (`uneven`), a second, shorter one shares the places that one each would leave
-// empty: 3000 tokens of 9000 keys 269 -> 222 us, six chunks of up to 300 of 2600 87 -> 70; beside many workgroups of
+// empty: 3000 tokens of 9000 keys 269 -> 230 us, six chunks of up to 300 of 2600 91 -> 75; beside many workgroups of
 // the other kind it loses (three of up to 300 and 20 tokens 63 -> 76), and so do a third and later chunk like it.
+// A second chunk of less than 0.3 of the first is level in the mean of 24 batches (3400 tokens of 9000 keys 270 -> 246,
+// 1658 tokens of 32 / 8 heads of 23335 686 -> 733) and costs partials: none then.
 PagedPart part_of(const PagedCall& c, int64_t tiles, int64_t there, int least, int whole, int64_t most, int64_t most_parts,
                   bool uneven) {
   const int64_t len = c.pb.max_len, rows = (int64_t)c.pb.tokens * c.hq;
@@ -163,9 +165,12 @@ void launch_rows(const PagedCall& c, const PagedPart& p, float* part) {
       INT32_MAX, p.chunk, p.used, p.used > 1 ? part : nullptr);
 }
 
-// Packed rows of a sequence up to which tiles of 32 rows take it rather than those of paged_tiles.hip: with 160 rows of
-// up to 8000 keys (four sequences) they are at 55 us and the others at 80, with 96 of 2000 at 19 against 32;
-// with 400 to 512 rows the large tiles come level (512 of 16384 keys: 59 us against 87).
+// Packed rows of a sequence up to which tiles of 32 rows take it rather than those of paged_tiles.hip.  Where the two meet
+// depends on the keys more than on the rows, and this is the middle.  Tiles of 32 rows against the others, us a call, of
+// chunks of as many tokens of 16 / 8 heads: over 2000 keys and fewer the small ones win on both sides of the limit (four
+// of 48: 27 against 29; of up to 132: 32 against 38; of up to 256: 34 against 36; sixteen of up to 132 of 500:
+// 26 against 47), over 8000 and more the large ones do (four of 80 of 8000: 65 against 57; of 100: 88 against 61; of
+// up to 256: 126 against 88; one of 256 of 16384: 89 against 60).
 constexpr int kFewRows = 256;
 
 template <typename T, int D>
@@ -176,8 +181,8 @@ int launch(const PagedCall& c) {
       sizeof(T) == 2 && most > kFewRows && c.st.kp == c.st.vp && c.st.kh == c.st.vh && c.st.kr == c.st.vr;
   const bool few_too = !many_too || c.pb.batch > 1;  // (a sequence alone is one or the other's)
   // Tiles of 256 rows read K and V half as often as those of 128, of which a CU holds two: better where one
-  // workgroup per CU is all there is and its keys are many (2048 tokens of 16384, 16 / 8 heads: 281 us against
-  // 317), worse with ragged or short ones (four chunks of 512 of 8192: 196 against 179).
+  // workgroup per CU is all there is and its keys are many (2048 tokens of 16384, 16 / 8 heads: 285 us against
+  // 318), worse with ragged or short ones (four chunks of 512 of 8192: 196 against 179).
   const int64_t tiles8 = many_too && !few_too ? tiles_of(c, 256) : 0;
   const int waves = tiles8 > 0 && tiles8 * c.hkv <= cus && c.pb.max_len >= 6144 ? 8 : 4;
   const int rt = most <= 16 ? 1 : 2;
@@ -199,8 +204,8 @@ int launch(const PagedCall& c) {
   // 512 keys of a tile at least: partials cost more than shorter chunks gain.  Beside a prompt's many rows, whose
   // workgroups take as long, few rows need no short chunks: partials of 2^18 rows at most.
   const int64_t places = cus * (waves == 8 ? 1 : 2);
-  // Few rows of up to 384 bf16 keys stay in one chunk: its third step costs less than the merge's launch (300 keys 7.8 us
-  // against 8.1, 200 keys 6.9 against 8.4; 450 keys 9.0 against 8.4; fp32 steps cost more: 200 keys 11.7 against 11.0).
+  // Few rows of up to 384 bf16 keys stay in one chunk: its third step costs less than the merge's launch (300 keys 7.9 us
+  // against 8.1, 200 keys 7.0 against 8.4; 450 keys 9.0 against 8.4; fp32 steps cost more: 200 keys 11.7 against 11.0).
   const PagedPart few =
       part_of(c, few_tiles, few_there, 128, sizeof(T) == 2 ? 384 : 128, cus * (sizeof(T) == 4 && D == 128 ? 1 : 2),
               many_too ? 1 << 18 : INT64_MAX, !many_too);

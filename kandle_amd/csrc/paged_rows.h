@@ -22,12 +22,12 @@ namespace kh {
 //     consecutive columns EPL r ..: 16 lanes read a whole row.  Tile dt of O^T has the columns EPL r + dt.
 // Nothing passes through LDS until the waves' (m, l, O) are joined at the end.
 //
-// Long caches: bound by HBM and by the lines a CU's L1 has in flight (8 bf16 sequences of 8k to 32k keys: 126 us,
-// 5.1 TB/s; a large copy moves 4.9).  Pages that sequences share come from L2 (four prompts' eight beams, 1531
-// keys: 20 us, 200 MB at 10 TB/s).  Short caches: the chain of length, page id, rows, products and join (two fp32
-// sequences of 777 keys: 9 us, one 32-key block per wave).  32 rows in fp32: the fp32 MFMAs of the longest tile
-// with one wave per SIMD (200 tokens of 1000: 49 us).  Cache hints on the loads gained nothing; 64 fp32 rows that
-// share K and V through LDS gained 3 to 18 % on long caches and lost 10 % on short ones.
+// Long caches: bound by the loads in flight and by uneven chunks (8 bf16 sequences of 8k to 32k keys: 127 us, 5.1 TB/s;
+// a large copy moves 4.9, the contiguous decode kernel reads 6.2).  Pages that sequences share come from L2 (four
+// prompts' eight beams, 1531 keys: 20 us, 200 MB at 10 TB/s).  Short caches: the chain of length, page id, rows, products
+// and join (two fp32 sequences of 777 keys: 9 us, one 32-key block per wave).  32 rows in fp32: the fp32 MFMAs of the
+// longest tile with one wave per SIMD (200 tokens of 1000: 49 us).  Cache hints on the loads gained nothing; 64 fp32 rows
+// that share K and V through LDS gained 3 to 18 % on long caches and lost 10 % on short ones.
 //
 // Softmax relative to a reference maximum m (raw q . k units) that the accumulators start from, raised
 // only when a lane's sum of P exceeds kSumMax, as in the contiguous prefill kernel: O / l does not depend on

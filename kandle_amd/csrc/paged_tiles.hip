@@ -15,8 +15,8 @@
 // blocks in no page, read as zeros).  K and V pools have equal strides here.
 //
 // Bound by the chain QK -> exp2 -> PV of each wave and by the uneven last tiles: 2048 tokens of 16384 keys (256-row
-// tiles) 272 us = 950 TFLOP/s, 70 % of a large matrix product; 64 sequences' chunks of 300 tokens of 5000
-// (128-row tiles) 710 TFLOP/s; 300 of 500, where a tile has six steps, 375.
+// tiles) 280 us a call, 9 of them the merge's = 940 TFLOP/s, 70 % of a large matrix product (a kernel trace, which
+// slows it, has 296 to 306 us); 64 sequences' chunks of 300 tokens of 5000 (128-row tiles) 770 TFLOP/s.
 #include "paged_rows.h"
 
 using namespace kh;
@@ -319,9 +319,8 @@ __global__ __launch_bounds__(WAVES * 64, MINB) void paged_tiles_kernel(
 }
 
 // Sequences of many rows and of few (chunks of prompts beside single tokens) in one launch, so that they run beside
-// each other: the first many.columns * many.used workgroups take tiles of 128 rows, the others of 32.  As two
-// launches one after the other six ragged chunks of up to 300 tokens took 88 us, four of 512 of 8192 179;
-// together 70 and 113.
+// each other: tiles of 128 rows and of 32.  As two launches one after the other six ragged chunks of up to 300 tokens take
+// 91 us, a chunk of 2048 of 8192 beside 31 tokens of 8192 394; together 75 and 275.
 template <int D>
 __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(const uint16_t* __restrict__ Q,
                                                              const uint16_t* __restrict__ K,
@@ -333,8 +332,8 @@ __global__ __launch_bounds__(256, 2) void paged_mixed_kernel(const uint16_t* __r
   constexpr int TILE = 4 * TileCfg<D, 4, 64>::STAGE, ROWS = 4 * RowLds<uint16_t, D, 2>::FLOATS;
   __shared__ __attribute__((aligned(16))) uint8_t lds[TILE > ROWS ? TILE : ROWS];
   __shared__ int odd[2][4];
-  // The two kinds take turns, one of each per CU, as long as both last.  (Chunk of 2048 rows of 8192 and 31 single
-  // tokens of 8192: 299 us, one kind after the other 374, turns of 8 workgroups 334.)
+  // The two kinds take turns, one of each per CU, as long as both last.  (Chunk of 2048 tokens of 8192 and 31 single
+  // tokens of 8192: 263 us, one kind after the other 268, turns of 64 workgroups 293, of 8 303.)
   const int of_many = many.columns * many.used, of_few = few.columns * few.used;
   const int both = min(of_many, of_few) / turn * turn;
   int x = blockIdx.x;
